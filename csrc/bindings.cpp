@@ -3002,7 +3002,10 @@ void latent_attention(torch::Tensor qa, torch::Tensor q, int64_t dim, int64_t ro
 }
 }  // namespace
 
+void bind_draft(pybind11::module_& m);   // draft_bindings.cpp
+
 PYBIND11_MODULE(_hip_kernels, m) {
+  bind_draft(m);
   m.def("rms_rows", &rms_rows, py::arg("x"), py::arg("w"), py::arg("y"), py::arg("eps"), py::arg("groups") = 1);
   m.def("norm_resadd", &norm_resadd, py::arg("y"), py::arg("w"), py::arg("eps"), py::arg("x"), py::arg("x_lp"),
         py::arg("groups") = 1, py::arg("bias") = py::none(), py::arg("x_wide") = py::none());

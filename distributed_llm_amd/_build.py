@@ -2,7 +2,7 @@
 travel with the repo snapshot to the GPU box.
 
   * ``ops/_hip_kernels*.so``  — gfx950 HIP kernels (csrc/kernels/*.hip) + torch bindings
-                                (csrc/bindings.cpp), compiled with ``hipcc --offload-arch=gfx950``.
+                                (csrc/*.cpp), compiled with ``hipcc --offload-arch=gfx950``.
   * ``engine/_runtime*.so``   — C++ serving runtime (csrc/runtime/*.cpp: paged-KV block manager with
                                 prefix-hash cache, scheduler core), g++ + pybind11, no GPU needed.
 
@@ -61,8 +61,8 @@ def build_hip(force: bool = False, jobs: int = 8) -> str:
     kdir = os.path.join(CSRC, "kernels")
     kernels = sorted(os.path.join(kdir, f) for f in os.listdir(kdir) if f.endswith(".hip"))
     headers = [os.path.join(kdir, f) for f in os.listdir(kdir) if f.endswith(".h")]
-    bind = os.path.join(CSRC, "bindings.cpp")
-    if not force and _newer(HIP_SO, kernels + headers + [bind]):
+    binds = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cpp"))
+    if not force and _newer(HIP_SO, kernels + headers + binds):
         return HIP_SO
     import torch
     from torch.utils import cpp_extension as ce
@@ -77,13 +77,13 @@ def build_hip(force: bool = False, jobs: int = 8) -> str:
     for src in kernels:
         obj = os.path.join(BUILD, os.path.basename(src) + ".o")
         jobs_list.append([hipcc, *HIP_FLAGS, "-I", kdir, "-c", src, "-o", obj])
-    bind_obj = os.path.join(BUILD, "bindings.o")
-    jobs_list.append([hipcc, *HIP_FLAGS, *torch_inc, *py_inc, f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-                      "-DTORCH_EXTENSION_NAME=_hip_kernels", "-DTORCH_API_INCLUDE_EXTENSION_H",
-                      "-c", bind, "-o", bind_obj])
+    for bind in binds:
+        jobs_list.append([hipcc, *HIP_FLAGS, *torch_inc, *py_inc, f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+                          "-DTORCH_EXTENSION_NAME=_hip_kernels", "-DTORCH_API_INCLUDE_EXTENSION_H",
+                          "-c", bind, "-o", os.path.join(BUILD, os.path.basename(bind)[:-4] + ".o")])
     objs = [j[-1] for j in jobs_list]
     # incremental: an object newer than its source and every kernel header is reused
-    srcs = kernels + [bind]
+    srcs = kernels + binds
     todo = [j for j, src in zip(jobs_list, srcs) if force or not _newer(j[-1], [src] + headers)]
     with cf.ThreadPoolExecutor(max(1, min(jobs, len(todo) or 1))) as ex:
         list(ex.map(_run, todo))

@@ -839,3 +839,6 @@ def scatter_pairs(dst: torch.Tensor, buf: torch.Tensor) -> None:
             dst.view(-1)[pairs[:, 0]] = pairs[:, 1].to(dst.dtype)
         return
     ext.scatter_pairs(dst, buf)
+
+
+from . import draft, kv8  # noqa: E402,F401  (drafted tokens; the 8-bit cache)

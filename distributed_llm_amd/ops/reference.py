@@ -1142,3 +1142,165 @@ def gate_heads(o, gate, out):
     g = g.repeat_interleave(dv, 1) if g.shape[1] == H else g
     out.copy_((o.float().transpose(0, 1).reshape(T, H * dv) * g).to(out.dtype))
     return out
+
+
+# ----------------------------------------------------------------------------- 8-bit cache
+
+def kv8_quantise(x):
+    """e4m3 codes (as bytes) and f32 scales of the vectors in the last dimension of f32 ``x``: scale = top / 448, code = e4m3(448 x / top), top =
+    max |x| of at least 2^-100.  A vector with an infinity or NaN becomes NaN codes of scale 1."""
+    top = x.abs().amax(-1).clamp_min(2.0 ** -100)
+    odd = ~torch.isfinite(top)
+    code = (x * 0.875 / (top * 2.0 ** -9)[..., None]).clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(torch.uint8)
+    return torch.where(odd[..., None], 0x7F, code.int()).to(torch.uint8), torch.where(odd, 1.0, top / 448.0)
+
+
+def kv8_write(k, v, slots, cache):
+    sl = slots.long()
+    ok = (sl >= 0) & (sl < cache.k.shape[0] * BS)
+    blk, off = sl[ok] // BS, sl[ok] % BS
+    (ck, sk), (cv, sv) = kv8_quantise(k[ok].float()), kv8_quantise(v[ok].float())
+    cache.k.view(torch.uint8)[blk, :, off] = ck
+    cache.v.view(torch.uint8)[blk, :, :, off] = cv
+    cache.k_scale[blk, :, off], cache.v_scale[blk, :, off] = sk, sv
+
+
+def kv8_rope(qkv, positions, cos_sin, slots, cache, nq, nkv, d):
+    T = qkv.shape[0]
+    f = qkv[:, : (nq + 2 * nkv) * d].float().view(T, nq + 2 * nkv, d)
+    cs = cos_sin[positions.long().clamp(0, cos_sin.shape[0] - 1)].float()
+    rot = _rope(f[:, : nq + nkv], cs[:, : d // 2], cs[:, d // 2:])
+    kv8_write(rot[:, nq:], f[:, nq + nkv:], slots, cache)
+    return rot[:, :nq].to(qkv.dtype).contiguous()
+
+
+def kv8_read(cache, slots):
+    sl = slots.long()
+    ok = (sl >= 0) & (sl < cache.k.shape[0] * BS)
+    blk, off = torch.where(ok, sl, 0) // BS, torch.where(ok, sl, 0) % BS
+    k = cache.k.view(torch.uint8)[blk, :, off].view(torch.float8_e4m3fn).float() * cache.k_scale[blk, :, off][..., None]
+    v = cache.v.view(torch.uint8)[blk, :, :, off].view(torch.float8_e4m3fn).float() * cache.v_scale[blk, :, off][..., None]
+    return [torch.where(ok[:, None, None], x, 0.0).bfloat16() for x in (k, v)]
+
+
+# ----------------------------------------------------------------------------- drafted tokens
+
+def tree_mask(parents, seq_qstart, seq_qlen, max_nodes):
+    T, W = parents.shape[0], (max_nodes + 31) // 32
+    mask, depth = torch.zeros(T, W, dtype=torch.int64), torch.zeros(T, dtype=torch.int32)
+    par = parents.tolist()
+    for q0, n in zip(seq_qstart.tolist(), seq_qlen.tolist()):
+        for i in range(min(n, 32 * W, T - q0) if 0 <= q0 else 0):
+            at, up = i, -1
+            while at >= 0:
+                mask[q0 + i, at // 32] |= 1 << (at % 32)
+                up += 1
+                at = par[q0 + at] if par[q0 + at] < at else -1
+            depth[q0 + i] = up
+    return torch.where(mask >= 1 << 31, mask - (1 << 32), mask).to(torch.int32), depth
+
+
+def tree_attention(q, k_cache, v_cache, block_tables, seq_qstart, seq_qlen, seq_ctx, mask, scale, k_scale=None, v_scale=None):
+    """Sequence by sequence; 64-bit queries are computed in 64 bits."""
+    T, nq, d = q.shape
+    nb, nkv = k_cache.shape[:2]
+    G, wide = nq // nkv, torch.float64 if q.dtype == torch.float64 else torch.float32
+    out = torch.zeros_like(q)
+    for s in range(block_tables.shape[0]):
+        q0, n = int(seq_qstart[s]), int(seq_qlen[s])
+        ctx = min(int(seq_ctx[s]), block_tables.shape[1] * BS)
+        rows = [i for i in range(n) if 0 <= q0 + i < T]
+        if not rows or ctx <= 0:
+            continue
+        pages = block_tables[s, : (ctx + BS - 1) // BS].long()
+        there = ((pages >= 0) & (pages < nb)).repeat_interleave(BS)[:ctx]
+        pages = torch.where((pages >= 0) & (pages < nb), pages, 0)
+        k, v = [(c.view(torch.uint8)[pages].view(c.dtype) if c.dtype == torch.float8_e4m3fn else c[pages]).to(wide) for c in (k_cache, v_cache)]
+        if k_scale is not None:
+            k, v = k * k_scale[pages].to(wide)[..., None], v * v_scale[pages].to(wide)[:, :, None]
+        k, v = k.permute(1, 0, 2, 3).reshape(nkv, -1, d)[:, :ctx], v.permute(1, 0, 3, 2).reshape(nkv, -1, d)[:, :ctx]
+        j, base = torch.arange(ctx, device=q.device), ctx - n
+        for i in rows:
+            if mask is None:
+                see = j <= base + i
+            else:
+                at = j - base
+                word = mask[q0 + i].long()[(at // 32).clamp(0, mask.shape[1] - 1)]
+                see = (at < 0) | ((at < 32 * mask.shape[1]) & ((word >> (at % 32)) & 1).bool())
+            see = see & there
+            if not bool(see.any()):
+                continue
+            x = q[q0 + i].to(wide).view(nkv, G, d)
+            w = torch.softmax((x @ k[:, see].transpose(1, 2)) * scale, -1)
+            out[q0 + i] = (w @ v[:, see]).reshape(nq, d).to(q.dtype)
+    return out
+
+
+def verify_drafts(target, tokens, uniform, seq_qstart, seq_qlen, max_nodes, parents=None, draft=None):
+    """One walk a sequence; products and sums in 64 bits."""
+    T, V = target.shape
+    S = seq_qstart.numel()
+    accepted, nxt = torch.zeros(S, dtype=torch.int32), torch.full((S,), -1, dtype=torch.int32)
+    path = torch.full((S, max_nodes), -1, dtype=torch.int32)
+    tok, u = tokens.tolist(), uniform.double().tolist()
+    for s, (q0, n) in enumerate(zip(seq_qstart.tolist(), seq_qlen.tolist())):
+        n = min(n, max_nodes)
+        if n <= 0 or q0 < 0 or q0 + n > T:
+            continue
+        par = [i - 1 if parents is None else int(parents[q0 + i]) for i in range(n)]
+        at, steps = 0, [0]
+        while True:
+            p = target[q0 + at].double()
+            kids = [i for i in range(at + 1, n) if par[i] == at]
+            took, gone, mass, w = None, set(), 1.0, p
+            for i in kids:
+                x = tok[q0 + i]
+                real = 0 <= x < V
+                px = float(p[x]) if real and x not in gone else 0.0
+                if draft is not None:
+                    ok = real and u[q0 + i] * float(draft[q0 + i, x]) < px
+                    w = p - draft[q0 + i].double()
+                else:
+                    ok = u[q0 + i] * mass < px
+                    mass -= px
+                    gone.add(x)
+                if ok:
+                    took = i
+                    break
+            if took is None:
+                break
+            at = took
+            steps.append(at)
+        if draft is None:
+            w = p.clone()
+            w[[x for x in gone if 0 <= x < V]] = 0.0
+        w = torch.where(w > 0, w, 0.0)
+        if not float(w.sum()) > 0:
+            w = torch.where(p > 0, p, 0.0)
+        run = w.cumsum(0)
+        over = (run > u[q0] * float(run[-1])).nonzero()
+        some = (w > 0).nonzero()
+        nxt[s] = int(over[0]) if over.numel() else int(some[-1]) if some.numel() else 0
+        accepted[s] = len(steps) - 1
+        path[s, : len(steps)] = torch.tensor(steps, dtype=torch.int32)
+    return accepted, nxt, path
+
+
+def keep_drafts(k_cache, v_cache, block_tables, seq_qlen, seq_ctx, path, accepted, k_scale=None, v_scale=None):
+    one = k_cache.dim() == 4
+    k, v, ks, vs = [t if t is None or not one else t[None] for t in (k_cache, v_cache, k_scale, v_scale)]
+    if ks is not None:
+        k, v = k.view(torch.uint8), v.view(torch.uint8)
+    nb, limit = k.shape[1], block_tables.shape[1] * BS
+    for s in range(block_tables.shape[0]):
+        n, base = int(seq_qlen[s]), int(seq_ctx[s]) - int(seq_qlen[s])
+        for to in range(1, min(int(accepted[s]), path.shape[1] - 1, n - 1) + 1):
+            node = int(path[s, to])
+            if not to < node < n or base + to < 0 or base + node >= limit:
+                continue
+            (a, i), (b, j) = [(int(block_tables[s, x // BS]), x % BS) for x in (base + node, base + to)]
+            if not (0 <= a < nb and 0 <= b < nb):
+                continue
+            k[:, b, :, j], v[:, b, :, :, j] = k[:, a, :, i].clone(), v[:, a, :, :, i].clone()
+            if ks is not None:
+                ks[:, b, :, j], vs[:, b, :, j] = ks[:, a, :, i].clone(), vs[:, a, :, i].clone()

@@ -11,7 +11,7 @@
 
 extern "C" {
 int dllm_tree_attention(const void*, long, long, const void*, const void*, const float*, const float*, const int*, const int*, const int*, const int*,
-                        const int*, void*, float*, float*, int, int, int, int, int, int, int, int, int, int, int, float, hipStream_t);
+                        const int*, void*, float*, float*, int, int, int, int, int, int, int, int, int, int, int, int, float, hipStream_t);
 int dllm_tree_mask(const int*, const int*, const int*, int*, int*, int, int, int, hipStream_t);
 int dllm_verify_parts(int, int*);
 int dllm_verify(const void*, long, const void*, long, int, const int*, const int*, const float*, const int*, const int*, int*, int*, int*, double*, int*,
@@ -123,23 +123,32 @@ Tensor tree_attention(Tensor q, Tensor k, Tensor v, Tensor bt, Tensor qstart, Te
   const int64_t G = nq / c.nkv;
   const int64_t most = std::min(max_qlen ? max_qlen : S == 1 ? T : W ? 32 * W : T, T) * G;
   const int64_t keys = std::min(max_ctx ? max_ctx : max_blocks * BS, max_blocks * BS);
-  const int rf = most <= 16 ? 1 : most <= 32 ? 2 : 4;
-  int64_t nwg = (int64_t)cus(q) * 2 / 8 * 8;
-  const int64_t blocks = S * c.nkv * ((most + 16 * rf - 1) / (16 * rf));      // row blocks, at most
-  const int64_t ulen = keys > 256 ? 256 : 0;
+  int rf = most <= 16 ? 1 : most <= 32 ? 2 : 3;
+  if (getenv("T_RF")) rf = atoi(getenv("T_RF"));
+  int64_t mul = getenv("T_MUL") ? atoi(getenv("T_MUL")) : 2;
+  int64_t nwg = (int64_t)cus(q) * mul / 8 * 8;
+  const int64_t R = 16 * rf;
+  const int64_t blocks = S * c.nkv * ((most + R - 1) / R);      // row blocks, at most
+  int64_t ulen = keys > 256 ? 256 : 0;
+  if (getenv("T_UL")) { ulen = atoi(getenv("T_UL")); if (ulen >= keys) ulen = 0; }
+  // the list of units is counted in 32 bits
+  const int64_t listed = c.nkv * (T * G / R + S);
+  NEED(T * nq <= 0x7fffffff && listed < (1 << 30), "tree_attention: too many");
+  while (ulen && listed * (max_blocks * BS / ulen + 1) >= (1 << 30)) ulen *= 2;
   nwg = std::min(nwg, (blocks * (ulen ? (keys + ulen - 1) / ulen : 1) + 7) / 8 * 8);
   Tensor part;
   float *po = nullptr, *pml = nullptr;
   if (ulen) {
-    const int64_t rows = 2 * nwg * 16 * rf;
+    const int64_t rows = 2 * nwg * R;
     part = at::empty({rows * (d + 2)}, q.options().dtype(at::kFloat));
     po = part.data_ptr<float>();
     pml = po + rows * d;
   }
+  const int64_t join_rows = std::min<int64_t>(R, (most + 3) / 4 * 4);
   launched(dllm_tree_attention(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), ks ? ks->data_ptr<float>() : nullptr,
                                vs ? vs->data_ptr<float>() : nullptr, bt.data_ptr<int>(), qstart.data_ptr<int>(), qlen.data_ptr<int>(), ctx.data_ptr<int>(),
                                mask ? mask->data_ptr<int>() : nullptr, o.data_ptr(), po, pml, (int)W, (int)S, (int)T, (int)nq, (int)c.nkv, (int)d,
-                               (int)max_blocks, (int)c.blocks, (int)nwg, (int)ulen, rf, (float)scale, stream()),
+                               (int)max_blocks, (int)c.blocks, (int)nwg, (int)ulen, rf, (int)join_rows, (float)scale, stream()),
            "tree_attention");
   return o;
 }

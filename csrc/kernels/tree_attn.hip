@@ -22,7 +22,7 @@
 
 namespace {
 constexpr int BS = 16, NW = 4;
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, SLACK = 8.f;
 
 struct TreeArgs {
   const u16* q;             // [T, nq, d], token and head strides
@@ -38,63 +38,59 @@ struct TreeArgs {
   float scale_log2;
 };
 
-// ---- the list of units
-struct Place {
-  int seq;                  // sequence, and unit within it, of one place in the list
-  long local;
-};
+// ---- the list of units (32-bit: the launcher makes units long enough)
 struct Shape {
   int qlen, ctx, nb, nt;    // row blocks and key ranges
 };
 
 static __device__ __forceinline__ Shape shape_of(const TreeArgs& a, int s, int R) {
   Shape h;
-  h.qlen = max(a.qlen[s], 0);
+  h.qlen = min(max(a.qlen[s], 0), a.T);
   h.ctx = min(max(a.ctx[s], 0), a.max_blocks * BS);
-  h.nb = (int)(((long)h.qlen * a.G + R - 1) / R);
-  h.nt = max(1, (int)(((long)h.ctx + a.ulen - 1) / a.ulen));
+  h.nb = (h.qlen * a.G + R - 1) / R;
+  h.nt = a.ulen ? max(1, (h.ctx + a.ulen - 1) / a.ulen) : 1;
   return h;
 }
-static __device__ __forceinline__ long units_of(const TreeArgs& a, const Shape& h) { return (long)a.nkv * h.nb * h.nt; }
+static __device__ __forceinline__ int units_of(const TreeArgs& a, int s, int R) {
+  const Shape h = shape_of(a, s, R);
+  return a.nkv * h.nb * h.nt;
+}
+static __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// Units in all; each lane keeps the inclusive sum up to its own sequences.
-static __device__ __forceinline__ long scan_units(const TreeArgs& a, int R, long& incl, int& first, int& count) {
+// Where a unit of the list lies: a wave's scan over the sequences, each lane `count` neighbouring ones.  What the whole wave goes by is in
+// scalar registers.
+struct List {
+  int incl, first, count, total;
+};
+static __device__ __forceinline__ List scan_units(const TreeArgs& a, int R) {
   const int lane = threadIdx.x & 63;
-  count = (a.S + 63) / 64;
-  first = lane * count;
-  long own = 0;
-  for (int i = 0; i < count; ++i)
-    if (first + i < a.S) own += units_of(a, shape_of(a, first + i, R));
-  incl = own;
+  List q;
+  q.count = (a.S + 63) / 64;
+  q.first = lane * q.count;
+  q.incl = 0;
+  for (int i = 0; i < q.count; ++i)
+    if (q.first + i < a.S) q.incl += units_of(a, q.first + i, R);
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const long y = __shfl_up(incl, o, 64);
-    if (lane >= o) incl += y;
+    const int y = __shfl_up(q.incl, o, 64);
+    if (lane >= o) q.incl += y;
   }
-  return __shfl(incl, 63, 64);
+  q.total = __builtin_amdgcn_readlane(q.incl, 63);
+  return q;
 }
-static __device__ __forceinline__ Place place_of(const TreeArgs& a, int R, long incl, int first, int count, long unit) {
-  const unsigned long long at = __ballot(incl > unit);        // unit < total: some lane's
-  const int who = __builtin_ctzll(at);
-  int s = first;
-  long before = incl;
-  if ((int)(threadIdx.x & 63) == who) {
-    long own = 0;
-    for (int i = 0; i < count; ++i)
-      if (first + i < a.S) own += units_of(a, shape_of(a, first + i, R));
-    before -= own;
-    for (; s < a.S; ++s) {
-      const long n = units_of(a, shape_of(a, s, R));
-      if (before + n > unit) break;
-      before += n;
-    }
+// The sequence of `unit` (below the total), and its units' start.
+static __device__ __forceinline__ int place_of(const TreeArgs& a, int R, const List& q, int unit, int& start) {
+  const int who = __builtin_ctzll(__ballot(q.incl > unit));
+  int s = uniform(who * q.count), at = who ? __builtin_amdgcn_readlane(q.incl, who - 1) : 0;
+  for (; s < a.S - 1; ++s) {
+    const int n = uniform(units_of(a, s, R));
+    if (at + n > unit) break;
+    at += n;
   }
-  Place p;
-  p.seq = __builtin_amdgcn_readlane(s, who);
-  p.local = unit - __shfl(before, who, 64);
-  return p;
+  start = at;
+  return s;
 }
-static __device__ __forceinline__ long part_len(const TreeArgs& a, long total) { return (total + a.nwg - 1) / a.nwg; }
+static __device__ __forceinline__ int part_len(const TreeArgs& a, int total) { return uniform((total + a.nwg - 1) / a.nwg); }
 
 // ---- operands
 static __device__ __forceinline__ bf16x8 cvt8(uint2 r) {
@@ -108,18 +104,21 @@ static __device__ __forceinline__ bf16x8 cvt8(uint2 r) {
 }
 
 template <int D, int RF, bool EIGHT> struct Form {
-  static constexpr int CK = EIGHT && RF <= 2 ? 64 : 32;       // keys of a wave's chunk
+  static constexpr int CK = EIGHT && RF == 1 ? 64 : 32;       // keys of a wave's chunk
   static constexpr int KS = D / 32, NT = D / 16, TL = CK / 16, KPG = CK / 4, R = 16 * RF;
-  static constexpr bool QL = RF == 4;                         // Q fragments in LDS: their registers would cost a wave a SIMD
+  static constexpr bool QL = RF >= 3;                         // Q fragments in LDS: their registers would cost a wave a SIMD
   static constexpr int PITCH = D + 4;
 };
 
 template <int D, int RF, bool EIGHT> struct TreeSmem {
   using F = Form<D, RF, EIGHT>;
-  alignas(16) float o[NW][16][F::PITCH];
+  union {                                                     // the queries' place is the outputs' in the end
+    alignas(16) float o[NW][16][F::PITCH];
+    alignas(16) u16 q[F::QL ? RF * F::KS * 64 * 8 : 8];
+  };
   float m[NW][16], l[NW][16];
   alignas(16) float sc[EIGHT ? NW : 1][2][64];                // scales of a wave's chunk
-  alignas(16) u16 q[F::QL ? RF * F::KS * 64 * 8 : 8];
+  int odd;                                                    // infinities or NaN among V were left out
 };
 
 // Keys kb .. kb + 31 that a token sees, as bits.
@@ -139,23 +138,12 @@ static __device__ __forceinline__ uint32_t window(const TreeArgs& a, int kb, int
   return lim & ((lo >> sh) | hi);
 }
 
-template <bool EIGHT> static __device__ __forceinline__ bool odd_bits(uint32_t w) {     // an infinity or NaN among the values of a word
-  if (EIGHT) {
-    const uint32_t t = ~w & 0x7f7f7f7fu;                      // a byte that is 0 here is a NaN code
-    return ((t - 0x01010101u) & ~t & 0x80808080u) != 0;
-  }
-  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+// The top bit of every value of a word that is an infinity or NaN; and the word with those as zeros.
+template <bool EIGHT> static __device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
+  return EIGHT ? ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u : ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
 }
-template <bool EIGHT> static __device__ __forceinline__ uint32_t tame(uint32_t w) {     // those as zeros
-  if (EIGHT) {
-#pragma unroll
-    for (int b = 0; b < 32; b += 8)
-      if (((w >> b) & 0x7fu) == 0x7fu) w &= ~(0xffu << b);
-    return w;
-  }
-  if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
-  if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
-  return w;
+template <bool EIGHT> static __device__ __forceinline__ uint32_t tame(uint32_t w) {
+  return w & ~(EIGHT ? (odd_bits<true>(w) >> 7) * 0xffu : (odd_bits<false>(w) >> 15) * 0xffffu);
 }
 
 // Where a piece goes: the output, or slot `slot` of the workspace (< 0: the output).
@@ -163,44 +151,22 @@ template <int D, int RF, bool EIGHT>
 static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, EIGHT>& sm, const int seq, const Shape h, const int kvh, const int blk,
                                              const int k0, const int k1, const int slot) {
   using F = Form<D, RF, EIGHT>;
-  constexpr int CK = F::CK, KS = F::KS, NT = F::NT, TL = F::TL, KPG = F::KPG, R = F::R;
+  constexpr int CK = F::CK, KS = F::KS, NT = F::NT, TL = F::TL, KPG = F::KPG;
+  constexpr int KW = EIGHT ? 2 : 4, VW = EIGHT && CK == 32 ? 2 : 4;     // words of a lane's K step and V row
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, rl = lane & 15;
   const int qstart = a.qstart[seq], base = h.ctx - h.qlen;
   const int* bt = a.bt + (long)seq * a.max_blocks;
 
-  int tok[RF];
-  bool ok[RF];
-#pragma unroll
-  for (int f = 0; f < RF; ++f) {
-    const int r = blk * R + 16 * f + rl;
-    tok[f] = r / a.G;
-    const long at = (long)qstart + tok[f];
-    ok[f] = tok[f] < h.qlen && at >= 0 && at < a.T;
-  }
+  const int row0 = blk * F::R;
+  auto token = [&](int f) { return (row0 + 16 * f + rl) / a.G; };
+  auto real = [&](int t) { const long at = (long)qstart + t; return t < h.qlen && at >= 0 && at < a.T; };
   // Q fragments: dims 32 s + 8 g (bf16), or as the code loads deal them (pairs of steps share a 16-byte load)
   auto dim0 = [&](int s) { return EIGHT && (s | 1) < KS ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };
   auto q_at = [&](int f, int s) {
-    const int head = kvh * a.G + (blk * R + 16 * f + rl) % a.G;
-    return ok[f] ? ld16(a.q + (qstart + (long)tok[f]) * a.q_ts + head * a.q_hs + dim0(s)) : make_uint4(0u, 0u, 0u, 0u);
+    const int t = token(f), head = kvh * a.G + (row0 + 16 * f + rl) % a.G;
+    return real(t) ? ld16(a.q + (qstart + (long)t) * a.q_ts + head * a.q_hs + dim0(s)) : make_uint4(0u, 0u, 0u, 0u);
   };
-  bf16x8 qr[F::QL ? 1 : RF][KS];
-  if constexpr (F::QL) {
-    __syncthreads();                                          // the piece before is done with LDS
-#pragma unroll
-    for (int f = 0; f < RF; ++f)
-      if (f % NW == wave) {
-#pragma unroll
-        for (int s = 0; s < KS; ++s) st16(&sm.q[((f * KS + s) * 64 + lane) * 8], q_at(f, s));
-      }
-    __syncthreads();
-  } else {
-#pragma unroll
-    for (int f = 0; f < RF; ++f)
-#pragma unroll
-      for (int s = 0; s < KS; ++s) qr[f][s] = __builtin_bit_cast(bf16x8, q_at(f, s));
-  }
-
   f32x4 acc[RF][NT];
   float m[RF], l[RF];
 #pragma unroll
@@ -211,130 +177,155 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
     for (int n = 0; n < NT; ++n) acc[f][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  const int last_block = (h.ctx - 1) >> 4;
-  for (int kb = k0 + CK * wave; kb < k1; kb += CK * NW) {
-    // blocks of this lane's key rows and of its lane group's keys; a page outside the pool hides its keys
-    const int ik = min((kb >> 4) + (CK == 64 ? rl >> 2 : rl >> 3), last_block), iv = min((kb >> 4) + (CK == 64 ? g : g >> 1), last_block);
-    const int pk = bt[ik], pv = bt[iv];
-    const bool paged = (unsigned)pv < (unsigned)a.num_blocks;
-    const long hk = ((long)((unsigned)pk < (unsigned)a.num_blocks ? pk : 0) * a.nkv + kvh) * BS, hv = ((long)(paged ? pv : 0) * a.nkv + kvh) * BS;
-    uint32_t kr[TL][KS][EIGHT ? 2 : 4], vr[NT][EIGHT ? (CK == 64 ? 4 : 2) : 4];
+  // what a score is multiplied by on its way to the exponent (a scale of 0: the smallest that keeps -inf what it is)
+  const float c = EIGHT ? 1.f : fmaxf(fabsf(a.scale_log2), 0x1p-120f);
+
+  // A lane's pages: of its K rows and of its lane group's keys.  One outside the pool hides its keys.
+  const int last_block = (h.ctx - 1) >> 4, bk = CK == 64 ? rl >> 2 : rl >> 3, bv = CK == 64 ? g : g >> 1;
+  uint32_t kr[TL][KS][KW], vr[NT][VW];
+  float ks_l = 0.f, vs_l = 0.f;                               // e4m3: scales of key KPG g + rl of the chunk (rl < KPG)
+  int pk, pv, pk_n, pv_n;
+  auto pages = [&](int kb, int& to_k, int& to_v) {
+    to_k = bt[min((kb >> 4) + bk, last_block)];
+    to_v = bt[min((kb >> 4) + bv, last_block)];
+  };
+  auto in_pool = [&](int p) { return (unsigned)p < (unsigned)a.num_blocks; };
+  auto load_k = [&](int p) {
+    const long hk = ((long)(in_pool(p) ? p : 0) * a.nkv + kvh) * BS;
 #pragma unroll
     for (int t = 0; t < TL; ++t) {
       const long row = hk + (CK == 64 ? 0 : 8 * ((rl >> 2) & 1)) + 4 * t + (rl & 3);
       if constexpr (EIGHT) {
-        const uint8_t* p = (const uint8_t*)a.kc + row * D;
+        const uint8_t* x = (const uint8_t*)a.kc + row * D;
 #pragma unroll
         for (int s = 0; s < KS; s += 2) {
           if (s + 1 < KS) {
-            const uint4 v = ld16(p + 32 * s + 16 * g);
+            const uint4 v = ld16(x + 32 * s + 16 * g);
             kr[t][s][0] = v.x; kr[t][s][1] = v.y; kr[t][s + 1][0] = v.z; kr[t][s + 1][1] = v.w;
           } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(p + 32 * s + 8 * g);
+            const uint2 v = *reinterpret_cast<const uint2*>(x + 32 * s + 8 * g);
             kr[t][s][0] = v.x; kr[t][s][1] = v.y;
           }
         }
       } else {
-        const u16* p = (const u16*)a.kc + row * D + 8 * g;
+        const u16* x = (const u16*)a.kc + row * D + 8 * g;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          const uint4 v = ld16(p + 32 * s);
-          kr[t][s][0] = v.x; kr[t][s][1] = v.y; kr[t][s][2] = v.z; kr[t][s][3] = v.w;
+          const uint4 v = ld16(x + 32 * s);
+          kr[t][s][0] = v.x; kr[t][s][1] = v.y; kr[t][s][KW - 2] = v.z; kr[t][s][KW - 1] = v.w;
         }
+      }
+    }
+  };
+  auto load_v = [&](int kb, int p) {
+    const bool there = in_pool(p);
+    const long hv = ((long)(there ? p : 0) * a.nkv + kvh) * BS;
+    if constexpr (EIGHT) {
+      ks_l = vs_l = 0.f;
+      if (there && rl < KPG && kb + KPG * g + rl < h.ctx) {
+        const long at = hv + (CK == 64 ? rl : 8 * (g & 1) + rl);
+        ks_l = a.ks[at];
+        vs_l = a.vs[at];
       }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      if constexpr (EIGHT) {
-        const uint8_t* p = (const uint8_t*)a.vc + hv * D + (16 * n + rl) * BS;
-        if constexpr (CK == 64) {
-          const uint4 v = ld16(p);
-          vr[n][0] = v.x; vr[n][1] = v.y; vr[n][2] = v.z; vr[n][3] = v.w;
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(p + 8 * (g & 1));
-          vr[n][0] = v.x; vr[n][1] = v.y;
-        }
+      const uint8_t* x = (const uint8_t*)a.vc + (hv * D + (16 * n + rl) * BS) * (EIGHT ? 1 : 2) + (EIGHT ? (CK == 64 ? 0 : 8) : 16) * (g & 1);
+      if constexpr (VW == 4) {
+        const uint4 v = ld16(x);
+        vr[n][0] = v.x; vr[n][1] = v.y; vr[n][VW - 2] = v.z; vr[n][VW - 1] = v.w;
       } else {
-        const uint4 v = ld16((const u16*)a.vc + hv * D + (16 * n + rl) * BS + 8 * (g & 1));
-        vr[n][0] = v.x; vr[n][1] = v.y; vr[n][2] = v.z; vr[n][3] = v.w;
+        const uint2 v = *reinterpret_cast<const uint2*>(x);
+        vr[n][0] = v.x; vr[n][1] = v.y;
       }
     }
-    const bool plain = kb + CK <= base && !__any(!paged);     // every row sees the whole chunk
-    bool odd = false;
-    if constexpr (EIGHT) {
-      // key (lane) of the chunk: 16 keys of block iv, or 8 of one half
-      const int key = CK == 64 ? rl : 8 * (g & 1) + (rl & 7);
-      float ks = 0.f, vs = 0.f;
-      if (paged && kb + KPG * g + (CK == 64 ? rl : rl & 7) < h.ctx) { ks = a.ks[hv + key]; vs = a.vs[hv + key]; }
-      if (!plain && !(fabsf(vs) < INFINITY)) { odd = true; vs = 0.f; }
-      if (CK == 64 || rl < 8) {
-        sm.sc[wave][0][KPG * g + rl] = ks * a.scale_log2;
-        sm.sc[wave][1][KPG * g + rl] = vs;
+  };
+  auto k_frag = [&](int t, int s) {
+    if constexpr (EIGHT) return cvt8(make_uint2(kr[t][s][0], kr[t][s][1]));
+    else return __builtin_bit_cast(bf16x8, make_uint4(kr[t][s][0], kr[t][s][1], kr[t][s][KW - 2], kr[t][s][KW - 1]));
+  };
+  bf16x8 qr[F::QL ? 1 : RF][KS];
+  auto q_frag = [&](int f, int s) {
+    if constexpr (F::QL) return __builtin_bit_cast(bf16x8, ld16(&sm.q[((f * KS + s) * 64 + lane) * 8]));
+    else return qr[f][s];
+  };
+
+  // K of the next chunk is asked for as soon as the scores have used this one's registers, V as soon as the second product has, pages a chunk
+  // ahead of both: two chunks' latencies overlap without registers for two chunks.
+  int kb = k0 + CK * wave;
+  if (kb < k1) pages(kb, pk, pv);
+  if constexpr (F::QL) {
+#pragma unroll
+    for (int f = 0; f < RF; ++f)
+      if (f % NW == wave) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qr[0][s] = __builtin_bit_cast(bf16x8, q_at(f, s));
       }
-      __builtin_amdgcn_wave_barrier();
-    }
-    if (!plain) {
-      // what no row may see (keys past ctx, pages outside the pool: stale memory) is zero in V; an infinity or NaN of a drafted token that a
-      // row does not see would reach it as 0 * inf, so those are zero too and added again below, to the rows that see them
-      const int n = paged ? h.ctx - kb - KPG * g : 0;         // keys of this lane that exist
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int w = 0; w < (int)(sizeof(vr[0]) / 4); ++w) {
-          const int per = EIGHT ? 4 : 2, left = n - per * w;
-          uint32_t x = vr[i][w];
-          if (left < per) x &= left <= 0 ? 0u : (1u << ((EIGHT ? 8 : 16) * left)) - 1u;
-          odd |= odd_bits<EIGHT>(x);
-          vr[i][w] = tame<EIGHT>(x);
-        }
-    }
-    f32x4 sc[RF][TL];
+  } else {
 #pragma unroll
     for (int f = 0; f < RF; ++f)
 #pragma unroll
-      for (int t = 0; t < TL; ++t) sc[f][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < KS; ++s) qr[f][s] = __builtin_bit_cast(bf16x8, q_at(f, s));
+  }
+  if (kb < k1) {
+    load_k(pk);
+    load_v(kb, pv);
+    pages(kb + CK * NW, pk_n, pv_n);
+  }
+  __syncthreads();                                            // the piece before is done with LDS
+  if (threadIdx.x == 0) sm.odd = 0;
+  if constexpr (F::QL) {
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      bf16x8 kf[TL];
+    for (int f = 0; f < RF; ++f)
+      if (f % NW == wave) {
 #pragma unroll
-      for (int t = 0; t < TL; ++t) {
-        if constexpr (EIGHT) kf[t] = cvt8(make_uint2(kr[t][s][0], kr[t][s][1]));
-        else kf[t] = __builtin_bit_cast(bf16x8, make_uint4(kr[t][s][0], kr[t][s][1], kr[t][s][2], kr[t][s][3]));
+        for (int s = 0; s < KS; ++s) st16(&sm.q[((f * KS + s) * 64 + lane) * 8], __builtin_bit_cast(uint4, qr[0][s]));
       }
-#pragma unroll
-      for (int f = 0; f < RF; ++f) {
-        bf16x8 qf;
-        if constexpr (F::QL) qf = __builtin_bit_cast(bf16x8, ld16(&sm.q[((f * KS + s) * 64 + lane) * 8]));
-        else qf = qr[f][s];
-#pragma unroll
-        for (int t = 0; t < TL; ++t) sc[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t], qf, sc[f][t], 0, 0, 0);
+  }
+  __syncthreads();
+  for (int next; kb < k1; kb = next) {
+    next = kb + CK * NW;
+    const bool paged = in_pool(pv);
+    const bool plain = kb + CK <= base && !__any(!paged);     // every row sees the whole chunk
+    bool odd = false;
+    if constexpr (EIGHT) {
+      if (!plain && !(fabsf(vs_l) < INFINITY)) { odd = true; vs_l = 0.f; }
+      if (rl < KPG) {
+        sm.sc[wave][0][KPG * g + rl] = ks_l * a.scale_log2;
+        sm.sc[wave][1][KPG * g + rl] = vs_l;
       }
+      __builtin_amdgcn_wave_barrier();
     }
     bf16x8 pf[RF][CK / 32];
-    uint32_t see[RF][CK / 32];
-#pragma unroll
-    for (int f = 0; f < RF; ++f) {
-      float p[KPG];
+    auto weigh = [&](int f, const f32x4* sc) {                // scores to weights, and the running maximum and sum
+      float p[KPG];                                           // in units of 1 / c of a power of two (e4m3: with the key's scale, c = 1)
 #pragma unroll
       for (int t = 0; t < TL; ++t) {
-        f32x4 ks = f32x4{a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
+        f32x4 ks = f32x4{1.f, 1.f, 1.f, 1.f};
         if constexpr (EIGHT) ks = *reinterpret_cast<const f32x4*>(&sm.sc[wave][0][KPG * g + 4 * t]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) p[4 * t + q] = sc[f][t][q] * ks[q];
+        for (int q = 0; q < 4; ++q) p[4 * t + q] = EIGHT ? sc[t][q] * ks[q] : sc[t][q];
+      }
+      if (!EIGHT && a.scale_log2 < 0.f) {
+#pragma unroll
+        for (int j = 0; j < KPG; ++j) p[j] = -p[j];
       }
       if (!plain) {
-#pragma unroll
-        for (int w = 0; w < CK / 32; ++w)
-          see[f][w] = ok[f] ? window(a, kb + 32 * w, base, h.ctx, tok[f], (long)qstart + tok[f]) : 0u;
-        const uint32_t mine = paged ? (CK == 64 ? see[f][g >> 1 & (CK / 32 - 1)] >> (16 * (g & 1)) : see[f][0] >> (8 * g)) : 0u;
+        int G = a.G;
+        asm volatile("" : "+s"(G));                           // (kept here: as loop invariants these were ten registers a row block)
+        const int t = (row0 + 16 * f + rl) / G;
+        // the lane's keys KPG g .. are inside one word of 32
+        const uint32_t mine = paged && real(t) ? window(a, kb + (CK == 64 ? 32 * (g >> 1) : 0), base, h.ctx, t, (long)qstart + t) >> (CK == 64 ? 16 * (g & 1) : 8 * g) : 0u;
 #pragma unroll
         for (int j = 0; j < KPG; ++j) p[j] = (mine >> j) & 1u ? p[j] : -INFINITY;
       }
       float top = p[0];
 #pragma unroll
       for (int j = 1; j < KPG; ++j) top = fmaxf(top, p[j]);
-      top = lane_max(lane_max(top, 16), 32);
-      if (__any(top > m[f])) {
+      // The sums' unit follows the maximum only where a score is 2^SLACK above it: weights of up to 2^SLACK lose nothing, and the exchange
+      // between lane groups and the pass over the sums are left out nearly always.
+      if (__any(top * c > m[f] + SLACK)) {
+        top = lane_max(lane_max(top, 16), 32) * c;
         const float m_new = fmaxf(m[f], top), al = __builtin_amdgcn_exp2f(m[f] - (m_new == -INFINITY ? 0.f : m_new));
         m[f] = m_new;
         l[f] *= al;
@@ -343,7 +334,7 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
       }
       const float ms = m[f] == -INFINITY ? 0.f : m[f];
 #pragma unroll
-      for (int j = 0; j < KPG; ++j) { p[j] = __builtin_amdgcn_exp2f(p[j] - ms); l[f] += p[j]; }
+      for (int j = 0; j < KPG; ++j) { p[j] = __builtin_amdgcn_exp2f(EIGHT ? p[j] - ms : fmaf(p[j], c, -ms)); l[f] += p[j]; }
       if constexpr (EIGHT) {
 #pragma unroll
         for (int t = 0; t < TL; ++t) {
@@ -354,40 +345,81 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
       }
 #pragma unroll
       for (int e = 0; e < CK / 32; ++e) pf[f][e] = __builtin_bit_cast(bf16x8, pack8(p + 8 * e));
+    };
+    if constexpr (EIGHT || !F::QL) {                          // a K step is converted once for all rows
+      f32x4 sc[RF][TL];
+#pragma unroll
+      for (int f = 0; f < RF; ++f)
+#pragma unroll
+        for (int t = 0; t < TL; ++t) sc[f][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        bf16x8 kf[TL];
+#pragma unroll
+        for (int t = 0; t < TL; ++t) kf[t] = k_frag(t, s);
+#pragma unroll
+        for (int f = 0; f < RF; ++f) {
+          const bf16x8 qf = q_frag(f, s);
+#pragma unroll
+          for (int t = 0; t < TL; ++t) sc[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t], qf, sc[f][t], 0, 0, 0);
+        }
+      }
+      if (next < k1) load_k(pk_n);
+#pragma unroll
+      for (int f = 0; f < RF; ++f) weigh(f, sc[f]);
+    } else {                                                  // bf16, 64 rows: sixteen rows' scores at a time
+#pragma unroll
+      for (int f = 0; f < RF; ++f) {
+        f32x4 sc[TL];
+#pragma unroll
+        for (int t = 0; t < TL; ++t) sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const bf16x8 qf = q_frag(f, s);
+#pragma unroll
+          for (int t = 0; t < TL; ++t) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k_frag(t, s), qf, sc[t], 0, 0, 0);
+        }
+        weigh(f, sc);
+      }
+      if (next < k1) load_k(pk_n);
+    }
+    if (!plain) {
+      // what no row may see (keys past ctx, pages outside the pool: stale memory) is zero in V; an infinity or NaN of a drafted token that a
+      // row does not see would reach it as 0 * inf, so those are zero too and added at the end, to the rows that see them
+      const int n = paged ? h.ctx - kb - KPG * g : 0;         // keys of this lane that exist
+      uint32_t real_w[VW], any = 0;
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        const int per = EIGHT ? 4 : 2, left = min(max(n - per * w, 0), per);
+        real_w[w] = left == per ? ~0u : (1u << ((EIGHT ? 8 : 16) * left)) - 1u;
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) any |= odd_bits<EIGHT>(vr[i][w] &= real_w[w]);
+      if (__any(any != 0 || odd)) {
+        sm.odd = 1;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vr[i][w] = tame<EIGHT>(vr[i][w]);
+      }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < CK / 32; ++e) {
         bf16x8 vf;
-        if constexpr (EIGHT) vf = cvt8(make_uint2(vr[n][2 * e], vr[n][2 * e + 1]));
-        else vf = __builtin_bit_cast(bf16x8, make_uint4(vr[n][0], vr[n][1], vr[n][2], vr[n][3]));
+        if constexpr (EIGHT) vf = cvt8(make_uint2(vr[n][(2 * e) % VW], vr[n][(2 * e + 1) % VW]));
+        else vf = __builtin_bit_cast(bf16x8, make_uint4(vr[n][0], vr[n][1], vr[n][VW - 2], vr[n][VW - 1]));
 #pragma unroll
         for (int f = 0; f < RF; ++f) acc[f][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[f][e], acc[f][n], 0, 0, 0);
       }
     if constexpr (EIGHT) __builtin_amdgcn_wave_barrier();     // scales are read before the next chunk's are written
-    if (!plain && __any(odd)) {
-      // infinities and NaN, key by key (rare): the values themselves, to the rows that see the key
-      for (int j = 0; j < CK && kb + j < h.ctx; ++j) {
-        const int page = bt[(kb + j) >> 4];
-        if ((unsigned)page >= (unsigned)a.num_blocks) continue;
-        const long at = ((long)page * a.nkv + kvh) * BS;
-        const int off = (kb + j) & 15;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const long i = at * D + (16 * n + 4 * g + r) * BS + off;
-            float v;
-            if constexpr (EIGHT) v = __builtin_amdgcn_cvt_f32_fp8(((const uint8_t*)a.vc)[i], 0) * a.vs[at + off];
-            else v = bf2f(((const u16*)a.vc)[i]);
-            if (!(fabsf(v) < INFINITY)) {
-#pragma unroll
-              for (int f = 0; f < RF; ++f)
-                if ((see[f][CK == 64 ? j >> 5 : 0] >> (j & 31)) & 1u) acc[f][n][r] += v;
-            }
-          }
-      }
+    if (next < k1) {
+      load_v(next, pv_n);
+      pv = pv_n;
+      pages(next + CK * NW, pk_n, pv_n);
     }
   }
 
@@ -402,141 +434,148 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
     __syncthreads();
     for (int e = 8 * threadIdx.x; e < 16 * D; e += 8 * 64 * NW) {
       const int row = e / D, col = e % D;
-      float w[NW], M = -INFINITY, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      float M = -INFINITY, L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < NW; ++i) M = fmaxf(M, sm.m[i][row]);
       const float Ms = M == -INFINITY ? 0.f : M;
 #pragma unroll
       for (int i = 0; i < NW; ++i) {
-        w[i] = __builtin_amdgcn_exp2f(sm.m[i][row] - Ms);
-        L += sm.l[i][row] * w[i];
+        const float c = __builtin_amdgcn_exp2f(sm.m[i][row] - Ms);
+        L += sm.l[i][row] * c;
         const f32x4 x = *reinterpret_cast<const f32x4*>(&sm.o[i][row][col]), y = *reinterpret_cast<const f32x4*>(&sm.o[i][row][col + 4]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { o[j] += x[j] * w[i]; o[4 + j] += y[j] * w[i]; }
+        for (int j = 0; j < 4; ++j) { o[j] += x[j] * c; o[4 + j] += y[j] * c; }
       }
+      const int of_block = f * 16 + row, r = row0 + of_block, t = r / a.G;
+      if (!real(t)) continue;
+      if (sm.odd)
+        for (int j = k0; j < k1; ++j) {                       // (rare) an infinity or NaN of V, to the rows that see it
+          const int page = bt[j >> 4];
+          if (!in_pool(page) || !(window(a, j, base, h.ctx, t, (long)qstart + t) & 1u)) continue;
+          const long at = ((long)page * a.nkv + kvh) * BS;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const long x = at * D + (col + c) * BS + (j & 15);
+            float v;
+            if constexpr (EIGHT) v = __builtin_amdgcn_cvt_f32_fp8(((const uint8_t*)a.vc)[x], 0) * a.vs[at + (j & 15)];
+            else v = bf2f(((const u16*)a.vc)[x]);
+            if (!(fabsf(v) < INFINITY)) o[c] += v;
+          }
+        }
       if (slot >= 0) {
-        const long at = (long)slot * R + 16 * f + row;
+        const long at = (long)slot * F::R + of_block;
         *reinterpret_cast<f32x4*>(a.part_o + at * D + col) = f32x4{o[0], o[1], o[2], o[3]};
         *reinterpret_cast<f32x4*>(a.part_o + at * D + col + 4) = f32x4{o[4], o[5], o[6], o[7]};
         if (col == 0) { a.part_ml[2 * at] = M; a.part_ml[2 * at + 1] = L; }
         continue;
       }
-      const int r = blk * R + 16 * f + row, t = r / a.G;
-      const long to = (long)qstart + t;
-      if (t >= h.qlen || to < 0 || to >= a.T) continue;
       const float inv = L == 0.f ? 0.f : 1.f / L;             // a row that sees nothing is zero
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j] *= inv;
-      st16(a.out + (to * a.nq + kvh * a.G + r % a.G) * D + col, pack8(o));
+      st16(a.out + ((qstart + (long)t) * a.nq + kvh * a.G + r % a.G) * D + col, pack8(o));
     }
   }
 }
 
+#ifndef MINW
+#define MINW(D, RF, EIGHT) (RF >= 2 ? 2 : D == 64 && !EIGHT ? 4 : D == 64 || D == 96 && !EIGHT ? 3 : 2)
+#endif
 template <int D, int RF, bool EIGHT>
-__global__ void __launch_bounds__(64 * NW, RF == 4 ? 2 : 1) tree_attn_kernel(TreeArgs a) {
+__global__ void __launch_bounds__(64 * NW, MINW(D, RF, EIGHT)) tree_attn_kernel(TreeArgs a) {
   using F = Form<D, RF, EIGHT>;
   __shared__ TreeSmem<D, RF, EIGHT> sm;
-  long incl;
-  int first, count;
-  const long total = scan_units(a, F::R, incl, first, count);
-  if (total == 0) return;
-  const long part = part_len(a, total);
+  const List q = scan_units(a, F::R);
+  if (q.total == 0) return;
+  const int part = part_len(a, q.total);
   // parts in the order of the list to workgroups of one XCD, whose L2 the row blocks of a kv head then share
-  const int parts = (int)((total + part - 1) / part), q8 = parts / 8, r8 = parts % 8, x = blockIdx.x % 8, i = blockIdx.x / 8;
+  const int parts = uniform((q.total + part - 1) / part), q8 = parts / 8, r8 = parts % 8, x = blockIdx.x % 8, i = blockIdx.x / 8;
   if (i >= q8 + (x < r8)) return;
-  const int me = x * q8 + min(x, r8) + i;
-  long u = me * part;
-  const long end = min(total, u + part);
-  Place p = place_of(a, F::R, incl, first, count, u);
-  int seq = p.seq;
-  long local = p.local;
-  bool begun = false;
+  const int me = x * q8 + min(x, r8) + i, end = min(q.total, (me + 1) * part);
+  int u = me * part, start, slot = 2 * me;
+  int seq = place_of(a, F::R, q, u, start);
   while (u < end) {
     const Shape h = shape_of(a, seq, F::R);
-    const long n = units_of(a, h);
-    if (local >= n) { ++seq; local = 0; continue; }           // (units are left, so a sequence with units follows)
-    const int range = (int)(local % h.nt), row = (int)(local / h.nt), blk = row % h.nb, kvh = row / h.nb;
-    const int take = (int)min((long)(h.nt - range), end - u);
-    const bool whole = range == 0 && take == h.nt;
-    const long k0 = (long)range * a.ulen, k1 = min((long)h.ctx, k0 + (long)take * a.ulen);
-    piece<D, RF, EIGHT>(a, sm, seq, h, kvh, blk, (int)k0, (int)k1, whole ? -1 : 2 * me + (begun ? 1 : 0));
-    begun = true;
+    const int n = uniform(a.nkv * h.nb * h.nt);
+    if (u - start >= n) { ++seq; start += n; continue; }      // (units are left, so a sequence with units follows)
+    const int nt = uniform(h.nt), nb = uniform(h.nb), row = uniform((u - start) / nt), range = u - start - row * nt;
+    const int kvh = uniform(row / nb), blk = row - kvh * nb, take = min(nt - range, end - u);
+    const int k0 = range * a.ulen, k1 = range + take == nt ? h.ctx : k0 + take * a.ulen;
+    piece<D, RF, EIGHT>(a, sm, seq, h, kvh, blk, k0, k1, take == nt ? -1 : slot);
+    slot = 2 * me + 1;
     u += take;
-    local += take;
   }
 }
 
 // Joins the pieces of one row block that several parts hold.  The workgroup of the first cut inside a block does it: part i's start is inside
-// block [b, b + nt) and part i - 1's is not.  blockIdx.y: sixteen rows of it, a wave a row at a time.
+// block [b, b + nt) and part i - 1's is not.
 template <int D>
 __global__ void __launch_bounds__(64 * NW) tree_join_kernel(TreeArgs a, int R) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  long incl;
-  int first, count;
-  const long total = scan_units(a, R, incl, first, count);
-  const long part = total ? part_len(a, total) : 1, cut = (long)(blockIdx.x + 1) * part;
-  if (cut >= total) return;
-  const Place p = place_of(a, R, incl, first, count, cut);
-  const Shape h = shape_of(a, p.seq, R);
-  const int range = (int)(p.local % h.nt), row = (int)(p.local / h.nt), blk = row % h.nb, kvh = row / h.nb;
-  const long b = cut - range;                                 // the row block's first unit
+  const List q = scan_units(a, R);
+  const int part = part_len(a, q.total), i0 = blockIdx.x;
+  if (q.total == 0 || (long)(i0 + 1) * part >= q.total) return;
+  const int cut = (i0 + 1) * part;
+  int start;
+  const int seq = place_of(a, R, q, cut, start);
+  const Shape h = shape_of(a, seq, R);
+  const int nt = uniform(h.nt), nb = uniform(h.nb), row = uniform((cut - start) / nt), range = cut - start - row * nt;
+  const int kvh = uniform(row / nb), blk = row - kvh * nb, b = cut - range;      // the row block's first unit
   if (range == 0 || cut - part > b) return;
-  const int i0 = blockIdx.x, i1 = (int)((b + h.nt - 1) / part), qstart = a.qstart[p.seq];
-  for (int r16 = wave; r16 < 16; r16 += NW) {
-    const int rr = 16 * blockIdx.y + r16, r = blk * R + rr, t = r / a.G;
+  const int i1 = uniform((b + nt - 1) / part), qstart = a.qstart[seq];
+  const int first = 2 * i0 + (i0 * part < b ? 1 : 0);         // part i0's piece of this block is its second where it began in another block
+  constexpr int LR = D / 4 <= 16 ? 16 : 32, RW = 64 * NW / LR;      // lanes of a row (four values each), rows at a time
+  const int lr = threadIdx.x % LR, col = min(4 * lr, D - 4);
+  for (int rr = RW * blockIdx.y + threadIdx.x / LR; rr < R; rr += RW * gridDim.y) {
+    const int r = blk * R + rr, t = r / a.G;
     const long to = (long)qstart + t;
     if (t >= h.qlen || to < 0 || to >= a.T) continue;
-    // part i0's piece of this block is its last one: its second where it began in another block
-    auto slot_row = [&](int i) { return ((long)2 * i + ((long)i * part < b ? 1 : 0)) * R + rr; };
-    float M = -INFINITY;
-    for (int i = i0 + lane; i <= i1; i += 64) M = fmaxf(M, a.part_ml[2 * slot_row(i)]);
-    M = wave_max(M);
+    auto slot_row = [&](int i) { return (long)(i == i0 ? first : 2 * i) * R + rr; };
+    float M = -INFINITY, L = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = i0; i <= i1; ++i) M = fmaxf(M, a.part_ml[2 * slot_row(i)]);
     const float Ms = M == -INFINITY ? 0.f : M;
-    float L = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll 4
     for (int i = i0; i <= i1; ++i) {
       const long at = slot_row(i);
       const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
       const float w = __builtin_amdgcn_exp2f(ml.x - Ms);
       L += ml.y * w;
-      if (2 * lane < D) {
-        const float2 x = *reinterpret_cast<const float2*>(a.part_o + at * D + 2 * lane);
-        o0 += x.x * w;
-        o1 += x.y * w;
-      }
+      o += *reinterpret_cast<const f32x4*>(a.part_o + at * D + col) * w;
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    if (2 * lane < D)
-      *reinterpret_cast<uint32_t*>(a.out + (to * a.nq + kvh * a.G + r % a.G) * D + 2 * lane) = f2bf2(o0 * inv, o1 * inv);
+    if (4 * lr < D)
+      *reinterpret_cast<uint2*>(a.out + (to * a.nq + kvh * a.G + r % a.G) * D + col) = make_uint2(f2bf2(o[0] * inv, o[1] * inv), f2bf2(o[2] * inv, o[3] * inv));
   }
 }
 
 template <int D, int RF, bool EIGHT> void launch(const TreeArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((tree_attn_kernel<D, RF, EIGHT>), dim3(a.nwg), dim3(64 * NW), 0, st, a);
 }
-template <int D> int launch_d(const TreeArgs& a, int rf, bool join, hipStream_t st) {
+template <int D> int launch_d(const TreeArgs& a, int rf, int rows, hipStream_t st) {
   const bool e = a.ks != nullptr;
   if (rf == 1) e ? launch<D, 1, true>(a, st) : launch<D, 1, false>(a, st);
   else if (rf == 2) e ? launch<D, 2, true>(a, st) : launch<D, 2, false>(a, st);
-  else e ? launch<D, 4, true>(a, st) : launch<D, 4, false>(a, st);
-  if (join && a.nwg > 1) hipLaunchKernelGGL((tree_join_kernel<D>), dim3(a.nwg - 1, rf), dim3(64 * NW), 0, st, a, 16 * rf);
+  else e ? launch<D, 3, true>(a, st) : launch<D, 3, false>(a, st);
+  if (a.ulen && a.nwg > 1) hipLaunchKernelGGL((tree_join_kernel<D>), dim3(a.nwg - 1, (rows + 15) / 16), dim3(64 * NW), 0, st, a, 16 * rf);
   return (int)hipGetLastError();
 }
 }  // namespace
 
-// rf: row blocks of 16 rf rows (1, 2, 4).  ulen: keys of a unit, a multiple of 256; 0: a row block is one unit (no workspace, one launch).
+// rf: a wave has 16 rf rows (1 to 3).  ulen: keys of a unit, a multiple of 256; 0: a row block is one unit (no workspace, one
+// launch).  rows: those of a block that the join's grid has waves for (a multiple of 4).
 extern "C" int dllm_tree_attention(const void* q, long q_ts, long q_hs, const void* kc, const void* vc, const float* ks, const float* vs,
                                    const int* bt, const int* qstart, const int* qlen, const int* ctx, const int* mask, void* out, float* part_o,
                                    float* part_ml, int W, int S, int T, int nq, int nkv, int d, int max_blocks, int num_blocks, int nwg, int ulen,
-                                   int rf, float scale, hipStream_t st) {
-  if (nkv < 1 || nq < nkv || nq % nkv || (rf != 1 && rf != 2 && rf != 4)) return -1;
+                                   int rf, int rows, float scale, hipStream_t st) {
+  if (nkv < 1 || nq < nkv || nq % nkv || rf < 1 || rf > 3 || rows < 4 || rows % 4 || rows > 16 * rf) return -1;
   if ((ks == nullptr) != (vs == nullptr) || S < 1 || T < 1 || max_blocks < 1 || num_blocks < 1 || nwg < 1) return -2;
   if (ulen < 0 || ulen % 256 || (ulen && (!part_o || !part_ml))) return -3;
   TreeArgs a{(const u16*)q, q_ts, q_hs, kc, vc, ks, vs, bt, qstart, qlen, ctx, mask, (u16*)out, part_o, part_ml,
-             W, S, T, nq, nkv, nq / nkv, max_blocks, num_blocks, nwg, ulen ? ulen : 0x7fffff00, scale * LOG2E};
+             W, S, T, nq, nkv, nq / nkv, max_blocks, num_blocks, nwg, ulen, scale * LOG2E};
   switch (d) {
-    case 64: return launch_d<64>(a, rf, ulen != 0, st);
-    case 96: return launch_d<96>(a, rf, ulen != 0, st);
-    case 128: return launch_d<128>(a, rf, ulen != 0, st);
+    case 64: return launch_d<64>(a, rf, rows, st);
+    case 96: return launch_d<96>(a, rf, rows, st);
+    case 128: return launch_d<128>(a, rf, rows, st);
   }
   return -4;
 }

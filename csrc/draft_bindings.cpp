@@ -11,7 +11,7 @@
 
 extern "C" {
 int dllm_tree_attention(const void*, long, long, const void*, const void*, const float*, const float*, const int*, const int*, const int*, const int*,
-                        const int*, void*, float*, float*, int, int, int, int, int, int, int, int, int, int, int, int, float, hipStream_t);
+                        const int*, void*, float*, float*, int*, int, int, int, int, int, int, int, int, int, int, int, int, int, float, hipStream_t);
 int dllm_tree_mask(const int*, const int*, const int*, int*, int*, int, int, int, hipStream_t);
 int dllm_verify_parts(int, int*);
 int dllm_verify(const void*, long, const void*, long, int, const int*, const int*, const float*, const int*, const int*, int*, int*, int*, double*, int*,
@@ -123,14 +123,18 @@ Tensor tree_attention(Tensor q, Tensor k, Tensor v, Tensor bt, Tensor qstart, Te
   const int64_t G = nq / c.nkv;
   const int64_t most = std::min(max_qlen ? max_qlen : S == 1 ? T : W ? 32 * W : T, T) * G;
   const int64_t keys = std::min(max_ctx ? max_ctx : max_blocks * BS, max_blocks * BS);
-  int rf = most <= 16 ? 1 : most <= 32 ? 2 : 3;
-  if (getenv("T_RF")) rf = atoi(getenv("T_RF"));
-  int64_t mul = getenv("T_MUL") ? atoi(getenv("T_MUL")) : 2;
-  int64_t nwg = (int64_t)cus(q) * mul / 8 * 8;
-  const int64_t R = 16 * rf;
+  // Rows of a wave, and whether four waves have rows of their own over shared keys (bf16).  us, sequences of 200 to 3000 keys, 8 kv heads of 128, one
+  // wave's 16 / 32 / 48 rows, four waves' 64 / 128: 48 rows 65 / 61 / 58, 54 / 63; 80 to 160 rows 163 / 117 / 115, 104 / 82; 512 rows of 8000 to 32000
+  // keys 940 / 389 / 327, 281 / 203.  e4m3 keys cost conversions in every wave that shares them, or LDS bandwidth as bf16: the last one 488 / 217 / 182
+  // and 286 / 211, 48 rows 46 / 41 / 37 and 43 / 51.
+  const bool wide = !c.eight && most > 32;
+  const int rf = wide ? (most <= 64 ? 1 : 2) : most <= 16 ? 1 : most <= 32 ? 2 : 3;
+  int64_t nwg = (int64_t)cus(q) * 2 / 8 * 8;      // two workgroups a CU (three: 70 -> 81 us for single tokens over 8 bits)
+  const int64_t R = 16 * rf * (wide ? 4 : 1);
   const int64_t blocks = S * c.nkv * ((most + R - 1) / R);      // row blocks, at most
-  int64_t ulen = keys > 256 ? 256 : 0;
-  if (getenv("T_UL")) { ulen = atoi(getenv("T_UL")); if (ulen >= keys) ulen = 0; }
+  // Keys of a unit: short ones share out short contexts evenly (1500 keys 49 us, 60 with 512), long ones leave fewer pieces to write and join
+  // (16000 keys, 96 rows 57 -> 45; 32000 keys of four sequences 191 -> 180).  What one unit holds is not split: one launch.
+  int64_t ulen = keys > 4096 ? 512 : keys > 256 ? 256 : 0;
   // the list of units is counted in 32 bits
   const int64_t listed = c.nkv * (T * G / R + S);
   NEED(T * nq <= 0x7fffffff && listed < (1 << 30), "tree_attention: too many");
@@ -138,17 +142,19 @@ Tensor tree_attention(Tensor q, Tensor k, Tensor v, Tensor bt, Tensor qstart, Te
   nwg = std::min(nwg, (blocks * (ulen ? (keys + ulen - 1) / ulen : 1) + 7) / 8 * 8);
   Tensor part;
   float *po = nullptr, *pml = nullptr;
+  int* joins = nullptr;
   if (ulen) {
     const int64_t rows = 2 * nwg * R;
-    part = at::empty({rows * (d + 2)}, q.options().dtype(at::kFloat));
+    part = at::empty({rows * (d + 2) + 8 * nwg + 1}, q.options().dtype(at::kFloat));
     po = part.data_ptr<float>();
     pml = po + rows * d;
+    joins = reinterpret_cast<int*>(pml + rows * 2);
   }
-  const int64_t join_rows = std::min<int64_t>(R, (most + 3) / 4 * 4);
+  const int64_t join_rows = std::min(R, most);
   launched(dllm_tree_attention(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), ks ? ks->data_ptr<float>() : nullptr,
                                vs ? vs->data_ptr<float>() : nullptr, bt.data_ptr<int>(), qstart.data_ptr<int>(), qlen.data_ptr<int>(), ctx.data_ptr<int>(),
-                               mask ? mask->data_ptr<int>() : nullptr, o.data_ptr(), po, pml, (int)W, (int)S, (int)T, (int)nq, (int)c.nkv, (int)d,
-                               (int)max_blocks, (int)c.blocks, (int)nwg, (int)ulen, rf, (int)join_rows, (float)scale, stream()),
+                               mask ? mask->data_ptr<int>() : nullptr, o.data_ptr(), po, pml, joins, (int)W, (int)S, (int)T, (int)nq, (int)c.nkv, (int)d,
+                               (int)max_blocks, (int)c.blocks, (int)nwg, (int)ulen, rf, wide, (int)join_rows, (float)scale, stream()),
            "tree_attention");
   return o;
 }

@@ -8,8 +8,9 @@
 // of CK: the K rows are dealt to the tiles for that (key CK / 4 * (m / 4) + 4 t + m % 4 is row m of tile t), which costs nothing, and makes a
 // lane's part of V^T one vector load (the V cache is stored transposed, 16 keys a block).
 //
-// A workgroup is four waves over the same RF * 16 rows (heads of one kv head, tokens x group), each with its own chunks: K and V go to
-// registers once for all rows and are never staged.  The waves meet in LDS at the end.
+// Few rows (up to 32; e4m3: any number, 48 at a time): a workgroup is four waves over the same 16 RF rows (heads of one kv head, tokens x group), each
+// with its own chunks.  K and V go to registers once for all rows and are never staged; the waves meet in LDS at the end.  Bound by memory: 64
+// single tokens of 500 to 6000 keys, 8 kv heads of 128, 114 us (5.1 TB/s), over e4m3 68 (4.4).  More rows: tree_wide_kernel below.
 //
 // e4m3 caches: codes become bf16 exactly (three bits behind the leading one), the key's scale multiplies its score and the value's its weight,
 // ahead of the weight's rounding to bf16; the sum of weights is of the unrounded ones.
@@ -34,6 +35,7 @@ struct TreeArgs {
   const int* mask;          // [T, W] or null
   u16* out;                 // [T, nq, d]
   float *part_o, *part_ml;  // [2 nwg, R, d], [2 nwg, R, 2]
+  int* joins;               // [nwg, 8]: what the join has to do for a part that begins a block others end; [nwg]: the number of parts
   int W, S, T, nq, nkv, G, max_blocks, num_blocks, nwg, ulen;
   float scale_log2;
 };
@@ -93,6 +95,7 @@ static __device__ __forceinline__ int place_of(const TreeArgs& a, int R, const L
 static __device__ __forceinline__ int part_len(const TreeArgs& a, int total) { return uniform((total + a.nwg - 1) / a.nwg); }
 
 // ---- operands
+static __device__ __forceinline__ uint4 flip(uint4 v, uint32_t sign) { return make_uint4(v.x ^ sign, v.y ^ sign, v.z ^ sign, v.w ^ sign); }
 static __device__ __forceinline__ bf16x8 cvt8(uint2 r) {
   typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
   union { bf2 p[4]; bf16x8 v; } u;
@@ -146,6 +149,105 @@ template <bool EIGHT> static __device__ __forceinline__ uint32_t tame(uint32_t w
   return w & ~(EIGHT ? (odd_bits<true>(w) >> 7) * 0xffu : (odd_bits<false>(w) >> 15) * 0xffffu);
 }
 
+// Which of a lane group's keys (CK / 4 of a chunk at kb) row `r` of a kv head's sees, as bits.
+template <int CK>
+static __device__ __forceinline__ uint32_t row_window(const TreeArgs& a, int kb, int base, int ctx, int r, int qlen, int qstart, int g) {
+  int G = a.G;
+  asm volatile("" : "+s"(G));                                 // (kept here: as loop invariants these were ten registers a row block)
+  const int t = r / G;
+  const long at = (long)qstart + t;
+  if (t >= qlen || at < 0 || at >= a.T) return 0u;
+  return window(a, kb + (CK == 64 ? 32 * (g >> 1) : 0), base, ctx, t, at) >> (CK == 64 ? 16 * (g & 1) : 8 * g);
+}
+
+// Scores times their keys' scales (e4m3), and what a row does not see at -inf.
+template <int RF, int TL, bool EIGHT> static __device__ __forceinline__ void scale_scores(f32x4 (&p)[RF][TL], const float* ks) {
+  if constexpr (EIGHT) {
+#pragma unroll
+    for (int t = 0; t < TL; ++t) {
+      const f32x4 k4 = *reinterpret_cast<const f32x4*>(ks + 4 * t);
+#pragma unroll
+      for (int f = 0; f < RF; ++f) p[f][t] *= k4;
+    }
+  }
+}
+template <int TL> static __device__ __forceinline__ void hide(f32x4 (&p)[TL], uint32_t mine) {
+#pragma unroll
+  for (int t = 0; t < TL; ++t)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) p[t][q] = (mine >> (4 * t + q)) & 1u ? p[t][q] : -INFINITY;
+}
+
+// Scores of a lane's rows to weights, with the running maximum m (of the exponent, c times the score) and sum l of each.  vs: the values' scales
+// (e4m3).
+template <int RF, int NT, int TL, bool EIGHT>
+static __device__ __forceinline__ void weights(f32x4 (&p)[RF][TL], const float* vs, float c, float (&m)[RF], float (&l)[RF], f32x4 (&acc)[RF][NT],
+                                               bf16x8 (&pf)[RF][TL / 2]) {
+  float top[RF];
+  bool up = false;
+#pragma unroll
+  for (int f = 0; f < RF; ++f) {
+    top[f] = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < TL; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) top[f] = fmaxf(top[f], p[f][t][q]);
+    up |= top[f] * c > m[f] + SLACK;
+  }
+  // The sums' unit follows the maximum only where a score is 2^SLACK above it: weights of up to 2^SLACK lose nothing, and the exchange between
+  // lane groups and the pass over the sums are left out nearly always.
+  if (__any(up)) {
+#pragma unroll
+    for (int f = 0; f < RF; ++f) {
+      const float m_new = fmaxf(m[f], lane_max(lane_max(top[f], 16), 32) * c), al = __builtin_amdgcn_exp2f(m[f] - (m_new == -INFINITY ? 0.f : m_new));
+      m[f] = m_new;
+      l[f] *= al;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) acc[f][n] *= al;
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < RF; ++f) {
+    const float ms = m[f] == -INFINITY ? 0.f : m[f];
+#pragma unroll
+    for (int t = 0; t < TL; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) { p[f][t][q] = __builtin_amdgcn_exp2f(fmaf(p[f][t][q], c, -ms)); l[f] += p[f][t][q]; }
+  }
+  if constexpr (EIGHT) {
+#pragma unroll
+    for (int t = 0; t < TL; ++t) {
+      const f32x4 v4 = *reinterpret_cast<const f32x4*>(vs + 4 * t);
+#pragma unroll
+      for (int f = 0; f < RF; ++f) p[f][t] *= v4;
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < RF; ++f)
+#pragma unroll
+    for (int e = 0; e < TL / 2; ++e)
+      pf[f][e] = __builtin_bit_cast(bf16x8, make_uint4(f2bf2(p[f][2 * e][0], p[f][2 * e][1]), f2bf2(p[f][2 * e][2], p[f][2 * e][3]),
+                                                       f2bf2(p[f][2 * e + 1][0], p[f][2 * e + 1][1]), f2bf2(p[f][2 * e + 1][2], p[f][2 * e + 1][3])));
+}
+
+// (rare) infinities and NaN of V among keys k0 .. k1 at N neighbouring dims from `col`, to a row that sees them
+template <int N, bool EIGHT, class O>
+static __device__ __forceinline__ void add_odd(const TreeArgs& a, const int* bt, int kvh, int D, int k0, int k1, int base, int ctx, int t, long row, int col, O&& o) {
+  for (int j = k0; j < k1; ++j) {
+    const int page = bt[j >> 4];
+    if ((unsigned)page >= (unsigned)a.num_blocks || !(window(a, j, base, ctx, t, row) & 1u)) continue;
+    const long at = ((long)page * a.nkv + kvh) * BS;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const long x = at * D + (col + i) * BS + (j & 15);
+      float v;
+      if constexpr (EIGHT) v = __builtin_amdgcn_cvt_f32_fp8(((const uint8_t*)a.vc)[x], 0) * a.vs[at + (j & 15)];
+      else v = bf2f(((const u16*)a.vc)[x]);
+      if (!(fabsf(v) < INFINITY)) o[i] += v;
+    }
+  }
+}
+
 // Where a piece goes: the output, or slot `slot` of the workspace (< 0: the output).
 template <int D, int RF, bool EIGHT>
 static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, EIGHT>& sm, const int seq, const Shape h, const int kvh, const int blk,
@@ -163,9 +265,10 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
   auto real = [&](int t) { const long at = (long)qstart + t; return t < h.qlen && at >= 0 && at < a.T; };
   // Q fragments: dims 32 s + 8 g (bf16), or as the code loads deal them (pairs of steps share a 16-byte load)
   auto dim0 = [&](int s) { return EIGHT && (s | 1) < KS ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };
+  const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;      // c below is positive
   auto q_at = [&](int f, int s) {
     const int t = token(f), head = kvh * a.G + (row0 + 16 * f + rl) % a.G;
-    return real(t) ? ld16(a.q + (qstart + (long)t) * a.q_ts + head * a.q_hs + dim0(s)) : make_uint4(0u, 0u, 0u, 0u);
+    return real(t) ? flip(ld16(a.q + (qstart + (long)t) * a.q_ts + head * a.q_hs + dim0(s)), sign) : make_uint4(0u, 0u, 0u, 0u);
   };
   f32x4 acc[RF][NT];
   float m[RF], l[RF];
@@ -177,8 +280,8 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
     for (int n = 0; n < NT; ++n) acc[f][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // what a score is multiplied by on its way to the exponent (a scale of 0: the smallest that keeps -inf what it is)
-  const float c = EIGHT ? 1.f : fmaxf(fabsf(a.scale_log2), 0x1p-120f);
+  // what a score is multiplied by on its way to the exponent (a scale of 0: a number that leaves -inf what it is)
+  const float c = fmaxf(fabsf(a.scale_log2), 0x1p-120f);
 
   // A lane's pages: of its K rows and of its lane group's keys.  One outside the pool hides its keys.
   const int last_block = (h.ctx - 1) >> 4, bk = CK == 64 ? rl >> 2 : rl >> 3, bv = CK == 64 ? g : g >> 1;
@@ -289,101 +392,38 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
     const bool plain = kb + CK <= base && !__any(!paged);     // every row sees the whole chunk
     bool odd = false;
     if constexpr (EIGHT) {
-      if (!plain && !(fabsf(vs_l) < INFINITY)) { odd = true; vs_l = 0.f; }
+      odd = !plain && !(fabsf(vs_l) < INFINITY);
+      if (odd) vs_l = 0.f;                                    // (what is seen is added at the end)
       if (rl < KPG) {
-        sm.sc[wave][0][KPG * g + rl] = ks_l * a.scale_log2;
+        sm.sc[wave][0][KPG * g + rl] = ks_l;
         sm.sc[wave][1][KPG * g + rl] = vs_l;
       }
       __builtin_amdgcn_wave_barrier();
     }
-    bf16x8 pf[RF][CK / 32];
-    auto weigh = [&](int f, const f32x4* sc) {                // scores to weights, and the running maximum and sum
-      float p[KPG];                                           // in units of 1 / c of a power of two (e4m3: with the key's scale, c = 1)
+    const float *ks = &sm.sc[EIGHT ? wave : 0][0][KPG * g], *vs = &sm.sc[EIGHT ? wave : 0][1][KPG * g];
+    f32x4 sc[RF][TL];
 #pragma unroll
-      for (int t = 0; t < TL; ++t) {
-        f32x4 ks = f32x4{1.f, 1.f, 1.f, 1.f};
-        if constexpr (EIGHT) ks = *reinterpret_cast<const f32x4*>(&sm.sc[wave][0][KPG * g + 4 * t]);
+    for (int f = 0; f < RF; ++f)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) p[4 * t + q] = EIGHT ? sc[t][q] * ks[q] : sc[t][q];
-      }
-      if (!EIGHT && a.scale_log2 < 0.f) {
+      for (int t = 0; t < TL; ++t) sc[f][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < KPG; ++j) p[j] = -p[j];
-      }
-      if (!plain) {
-        int G = a.G;
-        asm volatile("" : "+s"(G));                           // (kept here: as loop invariants these were ten registers a row block)
-        const int t = (row0 + 16 * f + rl) / G;
-        // the lane's keys KPG g .. are inside one word of 32
-        const uint32_t mine = paged && real(t) ? window(a, kb + (CK == 64 ? 32 * (g >> 1) : 0), base, h.ctx, t, (long)qstart + t) >> (CK == 64 ? 16 * (g & 1) : 8 * g) : 0u;
+    for (int s = 0; s < KS; ++s) {
+      bf16x8 kf[TL];
 #pragma unroll
-        for (int j = 0; j < KPG; ++j) p[j] = (mine >> j) & 1u ? p[j] : -INFINITY;
-      }
-      float top = p[0];
-#pragma unroll
-      for (int j = 1; j < KPG; ++j) top = fmaxf(top, p[j]);
-      // The sums' unit follows the maximum only where a score is 2^SLACK above it: weights of up to 2^SLACK lose nothing, and the exchange
-      // between lane groups and the pass over the sums are left out nearly always.
-      if (__any(top * c > m[f] + SLACK)) {
-        top = lane_max(lane_max(top, 16), 32) * c;
-        const float m_new = fmaxf(m[f], top), al = __builtin_amdgcn_exp2f(m[f] - (m_new == -INFINITY ? 0.f : m_new));
-        m[f] = m_new;
-        l[f] *= al;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[f][n] *= al;
-      }
-      const float ms = m[f] == -INFINITY ? 0.f : m[f];
-#pragma unroll
-      for (int j = 0; j < KPG; ++j) { p[j] = __builtin_amdgcn_exp2f(EIGHT ? p[j] - ms : fmaf(p[j], c, -ms)); l[f] += p[j]; }
-      if constexpr (EIGHT) {
-#pragma unroll
-        for (int t = 0; t < TL; ++t) {
-          const f32x4 vs = *reinterpret_cast<const f32x4*>(&sm.sc[wave][1][KPG * g + 4 * t]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) p[4 * t + q] *= vs[q];
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < CK / 32; ++e) pf[f][e] = __builtin_bit_cast(bf16x8, pack8(p + 8 * e));
-    };
-    if constexpr (EIGHT || !F::QL) {                          // a K step is converted once for all rows
-      f32x4 sc[RF][TL];
-#pragma unroll
-      for (int f = 0; f < RF; ++f)
-#pragma unroll
-        for (int t = 0; t < TL; ++t) sc[f][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        bf16x8 kf[TL];
-#pragma unroll
-        for (int t = 0; t < TL; ++t) kf[t] = k_frag(t, s);
-#pragma unroll
-        for (int f = 0; f < RF; ++f) {
-          const bf16x8 qf = q_frag(f, s);
-#pragma unroll
-          for (int t = 0; t < TL; ++t) sc[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t], qf, sc[f][t], 0, 0, 0);
-        }
-      }
-      if (next < k1) load_k(pk_n);
-#pragma unroll
-      for (int f = 0; f < RF; ++f) weigh(f, sc[f]);
-    } else {                                                  // bf16, 64 rows: sixteen rows' scores at a time
+      for (int t = 0; t < TL; ++t) kf[t] = k_frag(t, s);
 #pragma unroll
       for (int f = 0; f < RF; ++f) {
-        f32x4 sc[TL];
+        const bf16x8 qf = q_frag(f, s);
 #pragma unroll
-        for (int t = 0; t < TL; ++t) sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const bf16x8 qf = q_frag(f, s);
-#pragma unroll
-          for (int t = 0; t < TL; ++t) sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k_frag(t, s), qf, sc[t], 0, 0, 0);
-        }
-        weigh(f, sc);
+        for (int t = 0; t < TL; ++t) sc[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t], qf, sc[f][t], 0, 0, 0);
       }
-      if (next < k1) load_k(pk_n);
     }
+    if (next < k1) load_k(pk_n);
+    bf16x8 pf[RF][TL / 2];
+    scale_scores<RF, TL, EIGHT>(sc, ks);
     if (!plain) {
+#pragma unroll
+      for (int f = 0; f < RF; ++f) hide(sc[f], paged ? row_window<CK>(a, kb, base, h.ctx, row0 + 16 * f + rl, h.qlen, qstart, g) : 0u);
       // what no row may see (keys past ctx, pages outside the pool: stale memory) is zero in V; an infinity or NaN of a drafted token that a
       // row does not see would reach it as 0 * inf, so those are zero too and added at the end, to the rows that see them
       const int n = paged ? h.ctx - kb - KPG * g : 0;         // keys of this lane that exist
@@ -405,6 +445,7 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
           for (int w = 0; w < VW; ++w) vr[i][w] = tame<EIGHT>(vr[i][w]);
       }
     }
+    weights<RF, NT, TL, EIGHT>(sc, vs, c, m, l, acc, pf);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -448,20 +489,7 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
       }
       const int of_block = f * 16 + row, r = row0 + of_block, t = r / a.G;
       if (!real(t)) continue;
-      if (sm.odd)
-        for (int j = k0; j < k1; ++j) {                       // (rare) an infinity or NaN of V, to the rows that see it
-          const int page = bt[j >> 4];
-          if (!in_pool(page) || !(window(a, j, base, h.ctx, t, (long)qstart + t) & 1u)) continue;
-          const long at = ((long)page * a.nkv + kvh) * BS;
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const long x = at * D + (col + c) * BS + (j & 15);
-            float v;
-            if constexpr (EIGHT) v = __builtin_amdgcn_cvt_f32_fp8(((const uint8_t*)a.vc)[x], 0) * a.vs[at + (j & 15)];
-            else v = bf2f(((const u16*)a.vc)[x]);
-            if (!(fabsf(v) < INFINITY)) o[c] += v;
-          }
-        }
+      if (sm.odd) add_odd<8, EIGHT>(a, bt, kvh, D, k0, k1, base, h.ctx, t, (long)qstart + t, col, o);
       if (slot >= 0) {
         const long at = (long)slot * F::R + of_block;
         *reinterpret_cast<f32x4*>(a.part_o + at * D + col) = f32x4{o[0], o[1], o[2], o[3]};
@@ -477,57 +505,255 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
   }
 }
 
-#ifndef MINW
-#define MINW(D, RF, EIGHT) (RF >= 2 ? 2 : D == 64 && !EIGHT ? 4 : D == 64 || D == 96 && !EIGHT ? 3 : 2)
-#endif
-template <int D, int RF, bool EIGHT>
-__global__ void __launch_bounds__(64 * NW, MINW(D, RF, EIGHT)) tree_attn_kernel(TreeArgs a) {
-  using F = Form<D, RF, EIGHT>;
-  __shared__ TreeSmem<D, RF, EIGHT> sm;
-  const List q = scan_units(a, F::R);
-  if (q.total == 0) return;
+// A workgroup's part of the list: run(sequence, its shape, kv head, row block, first key, last key, slot) for every piece of it.
+template <class F> static __device__ __forceinline__ void walk(const TreeArgs& a, int R, F&& run) {
+  const List q = scan_units(a, R);
+  const bool lead = threadIdx.x == 0 && a.joins;
+  if (q.total == 0) {
+    if (lead && blockIdx.x == 0) a.joins[8 * a.nwg] = 0;
+    return;
+  }
   const int part = part_len(a, q.total);
   // parts in the order of the list to workgroups of one XCD, whose L2 the row blocks of a kv head then share
   const int parts = uniform((q.total + part - 1) / part), q8 = parts / 8, r8 = parts % 8, x = blockIdx.x % 8, i = blockIdx.x / 8;
   if (i >= q8 + (x < r8)) return;
   const int me = x * q8 + min(x, r8) + i, end = min(q.total, (me + 1) * part);
+  if (lead && me == 0) a.joins[8 * a.nwg] = parts;
+  if (lead) a.joins[8 * me] = -1;
   int u = me * part, start, slot = 2 * me;
-  int seq = place_of(a, F::R, q, u, start);
+  int seq = place_of(a, R, q, u, start);
   while (u < end) {
-    const Shape h = shape_of(a, seq, F::R);
+    const Shape h = shape_of(a, seq, R);
     const int n = uniform(a.nkv * h.nb * h.nt);
     if (u - start >= n) { ++seq; start += n; continue; }      // (units are left, so a sequence with units follows)
     const int nt = uniform(h.nt), nb = uniform(h.nb), row = uniform((u - start) / nt), range = u - start - row * nt;
     const int kvh = uniform(row / nb), blk = row - kvh * nb, take = min(nt - range, end - u);
     const int k0 = range * a.ulen, k1 = range + take == nt ? h.ctx : k0 + take * a.ulen;
-    piece<D, RF, EIGHT>(a, sm, seq, h, kvh, blk, k0, k1, take == nt ? -1 : slot);
+    if (lead && range == 0 && take < nt) {
+      int* to = a.joins + 8 * me;
+      to[0] = slot;
+      to[1] = (u + nt - 1) / part;
+      to[2] = blk * R;
+      to[3] = kvh;
+      to[4] = a.qstart[seq];
+      to[5] = h.qlen;
+    }
+    run(seq, h, kvh, blk, k0, k1, take == nt ? -1 : slot);
     slot = 2 * me + 1;
     u += take;
   }
 }
 
-// Joins the pieces of one row block that several parts hold.  The workgroup of the first cut inside a block does it: part i's start is inside
-// block [b, b + nt) and part i - 1's is not.
+template <int D, int RF, bool EIGHT>
+__global__ void __launch_bounds__(64 * NW, (RF > 1 || D > 64 ? 2 : EIGHT ? 3 : 4)) tree_attn_kernel(TreeArgs a) {
+  __shared__ TreeSmem<D, RF, EIGHT> sm;
+  walk(a, Form<D, RF, EIGHT>::R, [&](int seq, const Shape& h, int kvh, int blk, int k0, int k1, int slot) __attribute__((always_inline)) {
+    piece<D, RF, EIGHT>(a, sm, seq, h, kvh, blk, k0, k1, slot);
+  });
+}
+
+// ---- many rows: the waves have rows of their own and share the keys.
+// Four waves of 16 RF rows read every chunk from LDS, in two stages: a wave asks for its share of the next chunk, computes on this one and then writes
+// what has arrived.  One operand fragment is a kilobyte in lane order, read back as it lies, without conflicts.  K and V leave L2 once for 64 RF
+// rows: with rows of one wave only, every 48 read them again, and ragged trees of 80 to 160 rows (8 kv heads of 128, 32 sequences of 200 to 3000 keys)
+// ran at what L2 misses of four such readings allow.  (Loads straight to LDS made the compiler wait for all of them ahead of any LDS read.)
+template <int D, int RF> struct Wide {
+  static constexpr int CK = RF == 1 && D > 64 ? 32 : 64, KS = D / 32, NT = D / 16, TL = CK / 16, KPG = CK / 4, R = 16 * RF * NW;
+  // one-kilobyte slots of a stage: K a tile and 32 dims (slot t * KS + s), V eight keys a lane group and sixteen dims (KSL + e * NT + n)
+  static constexpr int KSL = TL * KS, SL = KSL + NT * (CK / 32), GI = SL / NW, PAGES = 1024;
+  static_assert(SL % NW == 0, "whole slots a wave");
+};
+template <int D, int RF> struct WideSmem {
+  using F = Wide<D, RF>;
+  alignas(16) unsigned char ring[2][F::SL * 1024];
+  int page[F::PAGES];                                         // from block `first` of the sequence on; -1: outside the pool
+  int odd;                                                    // infinities or NaN among V were left out
+};
+
+template <int D, int RF>
+static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D, RF>& sm, const int seq, const Shape h, const int kvh, const int blk,
+                                                  const int k0, const int k1, const int slot) {
+  using F = Wide<D, RF>;
+  constexpr int CK = F::CK, KS = F::KS, NT = F::NT, KPG = F::KPG;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, rl = lane & 15;
+  const int qstart = a.qstart[seq], base = h.ctx - h.qlen, row0 = (blk * NW + wave) * 16 * RF;
+  const int* bt = a.bt + (long)seq * a.max_blocks;
+  const bool idle = row0 >= h.qlen * a.G;                     // no row: this wave stages only
+  const int steps = (k1 - k0 + CK - 1) / CK, last_block = (h.ctx - 1) >> 4;
+  auto real = [&](int t) { const long at = (long)qstart + t; return t < h.qlen && at >= 0 && at < a.T; };
+
+  const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;      // c below is positive
+  bf16x8 qf[RF][KS];
+#pragma unroll
+  for (int f = 0; f < RF; ++f) {
+    const int r = row0 + 16 * f + rl, t = r / a.G, head = kvh * a.G + r % a.G;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      qf[f][s] = __builtin_bit_cast(bf16x8, real(t) ? flip(ld16(a.q + (qstart + (long)t) * a.q_ts + head * a.q_hs + 32 * s + 8 * g), sign) : make_uint4(0u, 0u, 0u, 0u));
+  }
+  int first = k0 >> 4;
+  auto fill = [&](int from) {
+    first = from;
+    for (int i = threadIdx.x; i < F::PAGES; i += 64 * NW) {
+      const int b = from + i, p = b <= last_block ? bt[b] : -1;
+      sm.page[i] = (unsigned)p < (unsigned)a.num_blocks ? p : -1;
+    }
+  };
+  __syncthreads();                                            // the piece before is done with LDS
+  if (threadIdx.x == 0) sm.odd = 0;
+  fill(first);
+  __syncthreads();
+
+  f32x4 acc[RF][NT];
+  float m[RF], l[RF];
+#pragma unroll
+  for (int f = 0; f < RF; ++f) {
+    m[f] = -INFINITY;
+    l[f] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[f][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  uint4 next[F::GI];                                          // this wave's share of a chunk
+  int next_real = 0;                                          // keys of this lane's that exist
+  bool next_plain = false;
+  auto load = [&](int i) {
+    const int kb = k0 + CK * i, at = (kb >> 4) - first;
+    const int pk = sm.page[at + (CK == 64 ? rl >> 2 : rl >> 3)], pv = sm.page[at + (CK == 64 ? g : g >> 1)];
+    const long hk = ((long)max(pk, 0) * a.nkv + kvh) * BS + (CK == 64 ? 0 : 8 * ((rl >> 2) & 1)) + (rl & 3), hv = ((long)max(pv, 0) * a.nkv + kvh) * BS;
+    next_plain = kb + CK <= base && !__any(pv < 0);
+    next_real = pv >= 0 ? h.ctx - kb - KPG * g : 0;
+#pragma unroll
+    for (int j = 0; j < F::GI; ++j) {
+      const int p = wave * F::GI + j;                         // uniform
+      const u16* src;
+      if (p < F::KSL) {
+        src = (const u16*)a.kc + (hk + 4 * (p / KS)) * D + 32 * (p % KS) + 8 * g;
+      } else {
+        const int v = p - F::KSL, n = v % NT, e = v / NT;
+        src = (const u16*)a.vc + (hv * D + (16 * n + rl) * BS) + (CK == 64 ? 8 * e : 8 * (g & 1));
+      }
+      next[j] = ld16(src);
+    }
+  };
+  auto store = [&](int i) {
+    unsigned char* ring = sm.ring[i & 1];
+    bool odd = false;
+    if (!next_plain) {
+      // what no row may see (keys past ctx, pages outside the pool: stale memory) is zero in V; an infinity or NaN of a drafted token that a
+      // row does not see would reach it as 0 * inf, so those are zero too and added at the end, to the rows that see them
+#pragma unroll
+      for (int j = 0; j < F::GI; ++j) {
+        const int v = wave * F::GI + j - F::KSL;
+        if (v < 0) continue;
+        uint32_t w[4] = {next[j].x, next[j].y, next[j].z, next[j].w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int left = min(max(next_real - 8 * (v / NT) - 2 * x, 0), 2);
+          w[x] &= left == 2 ? ~0u : (1u << (16 * left)) - 1u;
+          odd |= odd_bits<false>(w[x]) != 0;
+          w[x] = tame<false>(w[x]);
+        }
+        next[j] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      if (__any(odd)) sm.odd = 1;
+    }
+#pragma unroll
+    for (int j = 0; j < F::GI; ++j) st16(ring + (wave * F::GI + j) * 1024 + lane * 16, next[j]);
+  };
+  const float c = fmaxf(fabsf(a.scale_log2), 0x1p-120f);
+  if (steps > 0) { load(0); store(0); }
+  for (int i = 0; i < steps; ++i) {
+    const int kb = k0 + CK * i;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();                             // stage i is whole, and the other one free
+    asm volatile("" ::: "memory");
+    if (i + 1 < steps) {
+      if (((kb + 2 * CK) >> 4) - first > F::PAGES) {          // the window of pages moves on (uniform, every 16 PAGES keys)
+        fill(kb >> 4);
+        __syncthreads();
+      }
+      load(i + 1);
+    }
+    if (!idle) {
+    const unsigned char* ring = sm.ring[i & 1];
+    const bool paged = sm.page[(kb >> 4) - first + (CK == 64 ? g : g >> 1)] >= 0, plain = kb + CK <= base && !__any(!paged);
+#pragma unroll 1
+    for (int e = 0; e < CK / 32; ++e) {                       // tiles 2 e, 2 e + 1: eight neighbouring keys of a lane group's
+      f32x4 sc[RF][2];
+#pragma unroll
+      for (int f = 0; f < RF; ++f) sc[f][0] = sc[f][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const bf16x8 kf = __builtin_bit_cast(bf16x8, ld16(ring + ((2 * e + t2) * KS + s) * 1024 + lane * 16));
+#pragma unroll
+          for (int f = 0; f < RF; ++f) sc[f][t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[f][s], sc[f][t2], 0, 0, 0);
+        }
+      bf16x8 pf[RF][1];
+      if (!plain) {
+#pragma unroll
+        for (int f = 0; f < RF; ++f) hide(sc[f], paged ? row_window<CK>(a, kb, base, h.ctx, row0 + 16 * f + rl, h.qlen, qstart, g) >> (8 * e) : 0u);
+      }
+      weights<RF, NT, 2, false>(sc, nullptr, c, m, l, acc, pf);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, ld16(ring + (F::KSL + e * NT + n) * 1024 + lane * 16));
+#pragma unroll
+        for (int f = 0; f < RF; ++f) acc[f][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[f][0], acc[f][n], 0, 0, 0);
+      }
+    }
+    }
+    if (i + 1 < steps) store(i + 1);
+  }
+
+  // acc[f][n][r] = O^T[dim 16 n + 4 g + r][row 16 f + rl]: four neighbouring dims of the lane's own row
+  __syncthreads();
+  const bool any_odd = sm.odd != 0;
+#pragma unroll
+  for (int f = 0; f < RF; ++f) {
+    const float L = lane_add(lane_add(l[f], 16), 32);
+    const int r = row0 + 16 * f + rl, t = r / a.G;
+    if (!real(t)) continue;
+    const float inv = L == 0.f ? 0.f : 1.f / L;               // a row that sees nothing is zero
+    const long at = (long)slot * F::R + (wave * RF + f) * 16 + rl;
+    u16* to = a.out + ((qstart + (long)t) * a.nq + kvh * a.G + r % a.G) * D;
+    if (slot >= 0 && g == 0) { a.part_ml[2 * at] = m[f]; a.part_ml[2 * at + 1] = L; }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int col = 16 * n + 4 * g;
+      f32x4 o = acc[f][n];
+      if (any_odd) add_odd<4, false>(a, bt, kvh, D, k0, k1, base, h.ctx, t, (long)qstart + t, col, o);
+      if (slot >= 0) *reinterpret_cast<f32x4*>(a.part_o + at * D + col) = o;
+      else *reinterpret_cast<uint2*>(to + col) = make_uint2(f2bf2(o[0] * inv, o[1] * inv), f2bf2(o[2] * inv, o[3] * inv));
+    }
+  }
+}
+
+template <int D, int RF> __global__ void __launch_bounds__(64 * NW, 2) tree_wide_kernel(TreeArgs a) {
+  __shared__ WideSmem<D, RF> sm;
+  walk(a, Wide<D, RF>::R, [&](int seq, const Shape& h, int kvh, int blk, int k0, int k1, int slot) __attribute__((always_inline)) {
+    wide_piece<D, RF>(a, sm, seq, h, kvh, blk, k0, k1, slot);
+  });
+}
+
+// Joins the pieces of one row block that several parts hold: part blockIdx.x has its first keys (and left word of it), parts up to i1 the others as their
+// first pieces.
 template <int D>
 __global__ void __launch_bounds__(64 * NW) tree_join_kernel(TreeArgs a, int R) {
-  const List q = scan_units(a, R);
-  const int part = part_len(a, q.total), i0 = blockIdx.x;
-  if (q.total == 0 || (long)(i0 + 1) * part >= q.total) return;
-  const int cut = (i0 + 1) * part;
-  int start;
-  const int seq = place_of(a, R, q, cut, start);
-  const Shape h = shape_of(a, seq, R);
-  const int nt = uniform(h.nt), nb = uniform(h.nb), row = uniform((cut - start) / nt), range = cut - start - row * nt;
-  const int kvh = uniform(row / nb), blk = row - kvh * nb, b = cut - range;      // the row block's first unit
-  if (range == 0 || cut - part > b) return;
-  const int i1 = uniform((b + nt - 1) / part), qstart = a.qstart[seq];
-  const int first = 2 * i0 + (i0 * part < b ? 1 : 0);         // part i0's piece of this block is its second where it began in another block
+  const int i0 = blockIdx.x;
+  if (i0 >= a.joins[8 * a.nwg]) return;
+  const int* to_do = a.joins + 8 * i0;
+  const int first = to_do[0], i1 = to_do[1], row0 = to_do[2], kvh = to_do[3], qstart = to_do[4], qlen = to_do[5];
+  if (first < 0) return;
   constexpr int LR = D / 4 <= 16 ? 16 : 32, RW = 64 * NW / LR;      // lanes of a row (four values each), rows at a time
   const int lr = threadIdx.x % LR, col = min(4 * lr, D - 4);
   for (int rr = RW * blockIdx.y + threadIdx.x / LR; rr < R; rr += RW * gridDim.y) {
-    const int r = blk * R + rr, t = r / a.G;
+    const int r = row0 + rr, t = r / a.G;
     const long to = (long)qstart + t;
-    if (t >= h.qlen || to < 0 || to >= a.T) continue;
+    if (t >= qlen || to < 0 || to >= a.T) continue;
     auto slot_row = [&](int i) { return (long)(i == i0 ? first : 2 * i) * R + rr; };
     float M = -INFINITY, L = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -548,34 +774,38 @@ __global__ void __launch_bounds__(64 * NW) tree_join_kernel(TreeArgs a, int R) {
   }
 }
 
-template <int D, int RF, bool EIGHT> void launch(const TreeArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((tree_attn_kernel<D, RF, EIGHT>), dim3(a.nwg), dim3(64 * NW), 0, st, a);
-}
-template <int D> int launch_d(const TreeArgs& a, int rf, int rows, hipStream_t st) {
+template <int D> int launch_d(const TreeArgs& a, int rf, bool wide, int rows, hipStream_t st) {
   const bool e = a.ks != nullptr;
-  if (rf == 1) e ? launch<D, 1, true>(a, st) : launch<D, 1, false>(a, st);
-  else if (rf == 2) e ? launch<D, 2, true>(a, st) : launch<D, 2, false>(a, st);
-  else e ? launch<D, 3, true>(a, st) : launch<D, 3, false>(a, st);
-  if (a.ulen && a.nwg > 1) hipLaunchKernelGGL((tree_join_kernel<D>), dim3(a.nwg - 1, (rows + 15) / 16), dim3(64 * NW), 0, st, a, 16 * rf);
+  const dim3 grid(a.nwg), block(64 * NW);
+  if (wide && !e && rf == 1) hipLaunchKernelGGL((tree_wide_kernel<D, 1>), grid, block, 0, st, a);
+  else if (wide && !e && rf == 2) hipLaunchKernelGGL((tree_wide_kernel<D, 2>), grid, block, 0, st, a);
+  else if (wide) return -5;
+  else if (rf == 1 && e) hipLaunchKernelGGL((tree_attn_kernel<D, 1, true>), grid, block, 0, st, a);
+  else if (rf == 1) hipLaunchKernelGGL((tree_attn_kernel<D, 1, false>), grid, block, 0, st, a);
+  else if (rf == 2 && e) hipLaunchKernelGGL((tree_attn_kernel<D, 2, true>), grid, block, 0, st, a);
+  else if (rf == 2) hipLaunchKernelGGL((tree_attn_kernel<D, 2, false>), grid, block, 0, st, a);
+  else if (e) hipLaunchKernelGGL((tree_attn_kernel<D, 3, true>), grid, block, 0, st, a);
+  else return -5;
+  if (a.ulen && a.nwg > 1) hipLaunchKernelGGL((tree_join_kernel<D>), dim3(a.nwg - 1, (rows + 15) / 16), dim3(64 * NW), 0, st, a, 16 * rf * (wide ? NW : 1));
   return (int)hipGetLastError();
 }
 }  // namespace
 
-// rf: a wave has 16 rf rows (1 to 3).  ulen: keys of a unit, a multiple of 256; 0: a row block is one unit (no workspace, one
-// launch).  rows: those of a block that the join's grid has waves for (a multiple of 4).
+// rf: a wave has 16 rf rows (bf16 1 or 2, e4m3 up to 3).  wide (bf16): a row block is four waves' rows, else one's.  ulen: keys of a unit, a multiple of 256; 0: a row block is
+// one unit (no workspace, one launch).  rows: those of a block that the join's grid has waves for.
 extern "C" int dllm_tree_attention(const void* q, long q_ts, long q_hs, const void* kc, const void* vc, const float* ks, const float* vs,
                                    const int* bt, const int* qstart, const int* qlen, const int* ctx, const int* mask, void* out, float* part_o,
-                                   float* part_ml, int W, int S, int T, int nq, int nkv, int d, int max_blocks, int num_blocks, int nwg, int ulen,
-                                   int rf, int rows, float scale, hipStream_t st) {
-  if (nkv < 1 || nq < nkv || nq % nkv || rf < 1 || rf > 3 || rows < 4 || rows % 4 || rows > 16 * rf) return -1;
+                                   float* part_ml, int* joins, int W, int S, int T, int nq, int nkv, int d, int max_blocks, int num_blocks, int nwg, int ulen,
+                                   int rf, int wide, int rows, float scale, hipStream_t st) {
+  if (nkv < 1 || nq < nkv || nq % nkv || rf < 1 || rf > 3 || rows < 1) return -1;
   if ((ks == nullptr) != (vs == nullptr) || S < 1 || T < 1 || max_blocks < 1 || num_blocks < 1 || nwg < 1) return -2;
-  if (ulen < 0 || ulen % 256 || (ulen && (!part_o || !part_ml))) return -3;
+  if (ulen < 0 || ulen % 256 || (ulen && (!part_o || !part_ml || !joins))) return -3;
   TreeArgs a{(const u16*)q, q_ts, q_hs, kc, vc, ks, vs, bt, qstart, qlen, ctx, mask, (u16*)out, part_o, part_ml,
-             W, S, T, nq, nkv, nq / nkv, max_blocks, num_blocks, nwg, ulen, scale * LOG2E};
+             ulen ? joins : nullptr, W, S, T, nq, nkv, nq / nkv, max_blocks, num_blocks, nwg, ulen, scale * LOG2E};
   switch (d) {
-    case 64: return launch_d<64>(a, rf, rows, st);
-    case 96: return launch_d<96>(a, rf, rows, st);
-    case 128: return launch_d<128>(a, rf, rows, st);
+    case 64: return launch_d<64>(a, rf, wide, rows, st);
+    case 96: return launch_d<96>(a, rf, wide, rows, st);
+    case 128: return launch_d<128>(a, rf, wide, rows, st);
   }
   return -4;
 }

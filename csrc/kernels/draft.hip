@@ -107,20 +107,24 @@ static __device__ __forceinline__ void left_out(const VerifyArgs& a, VerifySmem&
   __syncthreads();
 }
 
-// Weights of the last draw at v .. v + 3: max(p - q, 0), exact in 64 bits; NaN counts as nothing.
-template <class T>
-static __device__ __forceinline__ void weights(const T* p, const T* q, int v, int V, bool vec, const VerifySmem& sm, double* w, double* pw) {
-  float f[4], h[4] = {0.f, 0.f, 0.f, 0.f};
-  if (v + 4 <= V) {
+// p and q at v .. v + 3, zeros from `end` on (a part's end, or the row's).
+template <class T> static __device__ __forceinline__ void fetch(const T* p, const T* q, int v, int end, bool vec, float* f, float* h) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = h[j] = 0.f;
+  if (v + 4 <= end) {
     val4(p + v, vec, f);
     if (q) val4(q + v, vec, h);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f[j] = v + j < V ? val<T>(p + v + j) : 0.f;
-      if (q) h[j] = v + j < V ? val<T>(q + v + j) : 0.f;
-    }
+    for (int j = 0; j < 4; ++j)
+      if (v + j < end) {
+        f[j] = val<T>(p + v + j);
+        if (q) h[j] = val<T>(q + v + j);
+      }
   }
+}
+// Weights of the last draw there: max(p - q, 0), exact in 64 bits; NaN counts as nothing.
+static __device__ __forceinline__ void weights(const float* f, const float* h, int v, const VerifySmem& sm, double* w, double* pw) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const double x = (double)f[j] - (double)h[j];
@@ -135,6 +139,10 @@ static __device__ __forceinline__ void weights(const T* p, const T* q, int v, in
   }
 }
 
+// v of lane j (uniform)
+static __device__ __forceinline__ double lane64(double v, int j) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), j), __builtin_amdgcn_readlane(__double2loint(v), j));
+}
 static __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
@@ -146,22 +154,10 @@ template <class T> static __device__ __forceinline__ bool vectors(const VerifyAr
   return !((uintptr_t)a.target & m) && !(a.target_ld * sizeof(T) & m) && !((uintptr_t)a.draft & m) && (!a.draft || !(a.draft_ld * sizeof(T) & m));
 }
 
-// The walk, in every workgroup of a sequence (a few dependent loads and LDS), then the weights' sum of this one's part of the vocabulary.
-// Node i is accepted where u q(x) < p(x) (drawn from q), or u m < p(x), m = 1 less what its earlier siblings held (given candidates): products
-// of f32 and f64 values, exact or rounded once, so a token does not hang on the order of sums.
-template <class T> __global__ void __launch_bounds__(NTH) verify_walk_kernel(VerifyArgs a) {
-  __shared__ VerifySmem sm;
-  const int s = blockIdx.y, tid = threadIdx.x, q0 = a.qstart[s];
-  int n = min(a.qlen[s], a.N);
-  if (q0 < 0 || q0 > a.T - n) n = 0;
-  if (n <= 0) {
-    if (blockIdx.x == 0) {
-      if (tid == 0) { a.accepted[s] = 0; a.found[((long)s * (a.P + 1) + a.P) * 2] = -1; }
-      for (int i = tid; i < a.N; i += NTH) a.path[(long)s * a.N + i] = -1;
-    }
-    return;
-  }
+// Where the accepted path ends, and its length, of more than 64 nodes: a thread a node, in LDS.
+template <class T> static __device__ __forceinline__ void tree_walk(const VerifyArgs& a, VerifySmem& sm, int q0, int n, int& last, int& len) {
   const T *target = (const T*)a.target, *draft = (const T*)a.draft;
+  const int tid = threadIdx.x;
   for (int i = tid; i < n; i += NTH) {
     const int p = parent_of(a, q0, i), x = a.tokens[q0 + i];
     sm.par[i] = p;
@@ -193,7 +189,7 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_walk_kernel(Ver
         double mass = 1.0;
         for (int j = sm.par[i] + 1; j < i; ++j)
           if (sm.par[j] == sm.par[i]) mass -= sm.px[j];
-        sm.ok[i] = (double)a.uniform[q0 + i] * mass < sm.px[i];
+        sm.ok[i] = sm.tok[i] >= 0 && sm.tok[i] < a.V && (double)a.uniform[q0 + i] * fmax(mass, 0.0) < sm.px[i];
       }
     __syncthreads();
   }
@@ -204,32 +200,95 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_walk_kernel(Ver
       if (is_first) sm.nxt[sm.par[i]] = i;
     }
   __syncthreads();
-  int last = 0, len = 1;
+  last = 0;
+  len = 1;
   for (int k = sm.nxt[0]; k >= 0; k = sm.nxt[k]) { last = k; ++len; }
-  bool mine = false;
-  for (int i = tid; i < n; i += NTH) mine |= sm.par[i] == last;
-  const bool refused = __syncthreads_or(mine);
-  if (blockIdx.x == 0) {
-    int* path = a.path + (long)s * a.N;
-    for (int i = len + tid; i < a.N; i += NTH) path[i] = -1;
-    if (tid == 0) {
-      for (int i = 0, k = 0; i < len; ++i, k = sm.nxt[k]) path[i] = k;
-      a.accepted[s] = len - 1;
-      int* f = a.found + ((long)s * (a.P + 1) + a.P) * 2;
-      f[0] = last;
-      f[1] = refused;
+}
+
+// The walk, in every workgroup of a sequence (a few dependent loads and LDS), then the weights' sum of this one's part of the vocabulary.
+// Node i is accepted where u q(x) < p(x) (drawn from q), or u m < p(x), m = 1 less what its earlier siblings held (given candidates): products
+// of f32 and f64 values, exact or rounded once, so a token does not hang on the order of sums.
+template <class T> __global__ void __launch_bounds__(NTH) verify_walk_kernel(VerifyArgs a) {
+  __shared__ VerifySmem sm;
+  const int s = blockIdx.y, tid = threadIdx.x, q0 = a.qstart[s];
+  int n = min(a.qlen[s], a.N);
+  if (q0 < 0 || q0 > a.T - n) n = 0;
+  if (n <= 0) {
+    if (blockIdx.x == 0) {
+      if (tid == 0) { a.accepted[s] = 0; a.found[((long)s * (a.P + 1) + a.P) * 2] = -1; }
+      for (int i = tid; i < a.N; i += NTH) a.path[(long)s * a.N + i] = -1;
     }
+    return;
   }
+  const T *target = (const T*)a.target, *draft = (const T*)a.draft;
+  int* path = a.path + (long)s * a.N;
+  int last = 0, len = 1;
+  bool refused;
   const int v0 = blockIdx.x * a.part, v1 = min(a.V, v0 + a.part);
-  left_out(a, sm, n, last, v0, v1);
+  if (n <= 64) {
+    // a lane a node, in every wave by itself, without LDS (trees of 40 nodes: 16 us of a launch in LDS, 11 so)
+    const int i = tid & 63, x = i < n ? a.tokens[q0 + i] : -1, par = i < n ? parent_of(a, q0, i) : -3;
+    const bool real = par >= 0 && x >= 0 && x < a.V;
+    double px = real ? (double)val<T>(target + (long)(q0 + par) * a.target_ld + x) : 0.0, mass = 1.0;
+    const double u = i < n ? (double)a.uniform[q0 + i] : 0.0;
+    if (a.parents)
+      for (int j = 1; j < n; ++j) {                                  // siblings in order: what each held, and tokens that come again
+        const int pj = __builtin_amdgcn_readlane(par, j), xj = __builtin_amdgcn_readlane(x, j);
+        const double held = lane64(px, j);
+        if (i > j && par == pj) {
+          mass -= held;
+          if (x == xj) px = 0.0;
+        }
+      }
+    bool take = real && (draft ? u * (double)val<T>(draft + (long)(q0 + i) * a.draft_ld + x) < px : u * fmax(mass, 0.0) < px);
+    for (unsigned long long m = __ballot(take); m; m &= m - 1) {     // a parent's first accepted child
+      const int j = __builtin_ctzll(m), pj = __builtin_amdgcn_readlane(par, j);
+      if (i > j && par == pj) take = false;
+    }
+    int step = 0;
+    for (unsigned long long m; (m = __ballot(take && par == last)) != 0; ++len) {
+      last = __builtin_ctzll(m);
+      if (i == len) step = last;
+    }
+    const unsigned long long kids = __ballot(par == last);
+    refused = kids != 0;
+    if (tid < 64) {
+      const unsigned long long out = draft ? 0ull : __ballot(par == last && x >= v0 && x < v1);
+      if (i == 0) sm.nout = __popcll(out);
+      if (out >> i & 1) sm.out[__popcll(out & ((1ull << i) - 1))] = x;
+      if (blockIdx.x == 0)
+        for (int j = i; j < a.N; j += 64) path[j] = j < len ? step : -1;
+    }
+    __syncthreads();
+  } else {
+    tree_walk<T>(a, sm, q0, n, last, len);
+    bool mine = false;
+    for (int i = tid; i < n; i += NTH) mine |= sm.par[i] == last;
+    refused = __syncthreads_or(mine);
+    if (blockIdx.x == 0) {
+      for (int i = len + tid; i < a.N; i += NTH) path[i] = -1;
+      if (tid == 0)
+        for (int i = 0, k = 0; i < len; ++i, k = sm.nxt[k]) path[i] = k;
+    }
+    left_out(a, sm, n, last, v0, v1);
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    a.accepted[s] = len - 1;
+    int* f = a.found + ((long)s * (a.P + 1) + a.P) * 2;
+    f[0] = last;
+    f[1] = refused;
+  }
   const T* p = target + (long)(q0 + last) * a.target_ld;
   const T* q = draft && refused ? draft + (long)(q0 + last + 1) * a.draft_ld : nullptr;
   const bool vec = vectors<T>(a);
   double ws = 0.0, ps = 0.0;
   int wl = -1, pl = -1;
+  // (four vectors asked for at once cost a workgroup on the CU: 17 us where this takes 13)
   for (int v = v0 + 4 * tid; v < v1; v += 4 * NTH) {
+    float f[4], h[4];
     double w[4], pw[4];
-    weights(p, q, v, a.V, vec, sm, w, pw);
+    fetch(p, q, v, v1, vec, f, h);
+    weights(f, h, v, sm, w, pw);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       ws += w[j];
@@ -270,7 +329,8 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_pick_kernel(Ver
     return;
   }
   const int q0 = a.qstart[s], n = min(a.qlen[s], a.N);
-  for (int i = tid; i < n; i += NTH) { sm.par[i] = parent_of(a, q0, i); sm.tok[i] = a.tokens[q0 + i]; }
+  if (!a.draft)
+    for (int i = tid; i < n; i += NTH) { sm.par[i] = parent_of(a, q0, i); sm.tok[i] = a.tokens[q0 + i]; }
   // parts (at most NTH): running sums, whole weights first
   const double* sums = a.sums + (long)s * a.P * 2;
   const int* lasts = a.found + (long)s * (a.P + 1) * 2;
@@ -291,14 +351,16 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_pick_kernel(Ver
     return x;
   };
   int which = 0;
-  double incl = scan(tid < a.P ? sums[2 * tid] : 0.0);
+  const double mine = tid < a.P ? sums[2 * tid] : 0.0, own_p = tid < a.P ? sums[2 * tid + 1] : 0.0;
+  const int last_w = tid < a.P ? lasts[2 * tid] : -1, last_p = tid < a.P ? lasts[2 * tid + 1] : -1;
+  double incl = scan(mine);
   if (!(cum[NTH - 1] > 0.0)) {
     which = 1;
     __syncthreads();
-    incl = scan(tid < a.P ? sums[2 * tid + 1] : 0.0);
+    incl = scan(own_p);
   }
   const double whole = cum[NTH - 1], t = (double)a.uniform[q0] * whole;
-  int l = tid < a.P ? lasts[2 * tid + which] : -1;
+  int l = which ? last_p : last_w;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) l = max(l, __shfl_xor(l, o, 64));
   if (lane == 0) sm.wlast[wid][0] = l;
@@ -322,11 +384,20 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_pick_kernel(Ver
   const T* q = a.draft && f[1] && !which ? (const T*)a.draft + (long)(q0 + last + 1) * a.draft_ld : nullptr;
   const bool vec = vectors<T>(a);
   const int from = v0 + tid * each, to = min(v1, from + each);
-  double own = 0.0;
-  for (int v = from; v < to; v += 4) {
-    double w[4], pw[4];
-    weights(p, q, v, a.V, vec, sm, w, pw);
-    own += w[0]; own += w[1]; own += w[2]; own += w[3];
+  // sixteen weights of a thread stay in registers; longer rows than 16 NTH NTH read theirs again
+  double w[16], pw[4], own = 0.0;
+  float f4[4][4], h4[4][4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) fetch(p, q, from + 4 * c, to, vec, f4[c], h4[c]);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) weights(f4[c], h4[c], from + 4 * c, sm, w + 4 * c, pw);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) own += w[j];
+  for (int v = from + 16; v < to; v += 4) {
+    double x[4];
+    fetch(p, q, v, to, vec, f4[0], h4[0]);
+    weights(f4[0], h4[0], v, sm, x, pw);
+    own += x[0]; own += x[1]; own += x[2]; own += x[3];
   }
   const double up = base + scan(own), down = tid ? base + cum[tid - 1] : base;
   if (tid == 0) pick = -1;
@@ -334,12 +405,16 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_pick_kernel(Ver
   if (up > t && !(down > t)) {
     double run = down;
     int got = -1;
-    for (int v = from; v < to; v += 4) {
-      double w[4], pw[4];
-      weights(p, q, v, a.V, vec, sm, w, pw);
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (w[j] > 0.0 && !(run > t)) { run += w[j]; got = from + j; }
+    for (int v = from + 16; v < to; v += 4) {
+      double x[4];
+      fetch(p, q, v, to, vec, f4[0], h4[0]);
+      weights(f4[0], h4[0], v, sm, x, pw);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (w[j] > 0.0 && !(run > t)) { run += w[j]; got = v + j; }
+        if (x[j] > 0.0 && !(run > t)) { run += x[j]; got = v + j; }
     }
     pick = got;
   }
@@ -355,6 +430,8 @@ struct KeepArgs {
   int L, S, N, nkv, d, max_blocks, num_blocks;
 };
 
+// V is a column of a transposed block, two bytes of every 32: a move touches lines of 32 d bytes for 2 d, which bounds it (32 sequences, 32 layers of 8 heads of
+// 128: 25 MB moved, about 200 touched, 30 us; four heads a workgroup 36).
 // A workgroup: one sequence, layer and kv head.  Path indices rise and node path[j] goes to place j <= path[j]: sixteen tokens at a time are
 // read, then written, and what is written lies ahead of every later source.  E: bytes of a value.
 template <int E> __global__ void __launch_bounds__(NTH) keep_kernel(KeepArgs a) {

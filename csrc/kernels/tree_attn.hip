@@ -45,51 +45,65 @@ struct Shape {
   int qlen, ctx, nb, nt;    // row blocks and key ranges
 };
 
-static __device__ __forceinline__ Shape shape_of(const TreeArgs& a, int s, int R) {
-  Shape h;
-  h.qlen = min(max(a.qlen[s], 0), a.T);
-  h.ctx = min(max(a.ctx[s], 0), a.max_blocks * BS);
-  h.nb = (h.qlen * a.G + R - 1) / R;
-  h.nt = a.ulen ? max(1, (h.ctx + a.ulen - 1) / a.ulen) : 1;
-  return h;
-}
-static __device__ __forceinline__ int units_of(const TreeArgs& a, int s, int R) {
-  const Shape h = shape_of(a, s, R);
-  return a.nkv * h.nb * h.nt;
-}
 static __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // Where a unit of the list lies: a wave's scan over the sequences, each lane `count` neighbouring ones.  What the whole wave goes by is in
 // scalar registers.
 struct List {
   int incl, first, count, total;
+  int qlen, ctx, qstart;    // of the lane's one sequence, where it has no more (up to 64 sequences: nothing is read twice)
 };
+static __device__ __forceinline__ Shape shape_of(const TreeArgs& a, int qlen, int ctx, int R) {
+  Shape h;
+  h.qlen = min(max(qlen, 0), a.T);
+  h.ctx = min(max(ctx, 0), a.max_blocks * BS);
+  h.nb = (h.qlen * a.G + R - 1) / R;
+  h.nt = a.ulen ? max(1, (h.ctx + a.ulen - 1) / a.ulen) : 1;
+  return h;
+}
+static __device__ __forceinline__ Shape shape_of(const TreeArgs& a, const List& q, int s, int R) {
+  if (q.count == 1) return shape_of(a, __builtin_amdgcn_readlane(q.qlen, s), __builtin_amdgcn_readlane(q.ctx, s), R);
+  return shape_of(a, a.qlen[s], a.ctx[s], R);
+}
+static __device__ __forceinline__ int qstart_of(const TreeArgs& a, const List& q, int s) {
+  return q.count == 1 ? __builtin_amdgcn_readlane(q.qstart, s) : a.qstart[s];
+}
 static __device__ __forceinline__ List scan_units(const TreeArgs& a, int R) {
   const int lane = threadIdx.x & 63;
   List q;
   q.count = (a.S + 63) / 64;
   q.first = lane * q.count;
   q.incl = 0;
-  for (int i = 0; i < q.count; ++i)
-    if (q.first + i < a.S) q.incl += units_of(a, q.first + i, R);
+  for (int i = 0; i < q.count; ++i) {
+    const int s = min(q.first + i, a.S - 1);
+    q.qlen = a.qlen[s];
+    q.ctx = a.ctx[s];
+    q.qstart = a.qstart[s];
+    const Shape h = shape_of(a, q.qlen, q.ctx, R);
+    if (q.first + i < a.S) q.incl += a.nkv * h.nb * h.nt;
+  }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(q.incl, o, 64);
-    if (lane >= o) q.incl += y;
+    if (o < a.S) {                                            // (lanes from S on only repeat the total)
+      const int y = __shfl_up(q.incl, o, 64);
+      if (lane >= o) q.incl += y;
+    }
   }
-  q.total = __builtin_amdgcn_readlane(q.incl, 63);
+  q.total = __builtin_amdgcn_readlane(q.incl, min(a.S, 64) - 1);
   return q;
 }
 // The sequence of `unit` (below the total), and its units' start.
 static __device__ __forceinline__ int place_of(const TreeArgs& a, int R, const List& q, int unit, int& start) {
   const int who = __builtin_ctzll(__ballot(q.incl > unit));
-  int s = uniform(who * q.count), at = who ? __builtin_amdgcn_readlane(q.incl, who - 1) : 0;
+  int s = uniform(who * q.count);
+  start = who ? __builtin_amdgcn_readlane(q.incl, who - 1) : 0;
+  if (q.count == 1) return s;
   for (; s < a.S - 1; ++s) {
-    const int n = uniform(units_of(a, s, R));
-    if (at + n > unit) break;
-    at += n;
+    const Shape h = shape_of(a, a.qlen[s], a.ctx[s], R);
+    const int n = uniform(a.nkv * h.nb * h.nt);
+    if (start + n > unit) break;
+    start += n;
   }
-  start = at;
   return s;
 }
 static __device__ __forceinline__ int part_len(const TreeArgs& a, int total) { return uniform((total + a.nwg - 1) / a.nwg); }
@@ -109,7 +123,7 @@ static __device__ __forceinline__ bf16x8 cvt8(uint2 r) {
 template <int D, int RF, bool EIGHT> struct Form {
   static constexpr int CK = EIGHT && RF == 1 ? 64 : 32;       // keys of a wave's chunk
   static constexpr int KS = D / 32, NT = D / 16, TL = CK / 16, KPG = CK / 4, R = 16 * RF;
-  static constexpr bool QL = RF >= 3;                         // Q fragments in LDS: their registers would cost a wave a SIMD
+  static constexpr bool QL = RF == 3 || (RF == 2 && D == 128 && !EIGHT);      // Q fragments in LDS: their registers would spill
   static constexpr int PITCH = D + 4;
 };
 
@@ -250,14 +264,14 @@ static __device__ __forceinline__ void add_odd(const TreeArgs& a, const int* bt,
 
 // Where a piece goes: the output, or slot `slot` of the workspace (< 0: the output).
 template <int D, int RF, bool EIGHT>
-static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, EIGHT>& sm, const int seq, const Shape h, const int kvh, const int blk,
+static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, EIGHT>& sm, const int seq, const int qstart, const Shape h, const int kvh, const int blk,
                                              const int k0, const int k1, const int slot) {
   using F = Form<D, RF, EIGHT>;
   constexpr int CK = F::CK, KS = F::KS, NT = F::NT, TL = F::TL, KPG = F::KPG;
   constexpr int KW = EIGHT ? 2 : 4, VW = EIGHT && CK == 32 ? 2 : 4;     // words of a lane's K step and V row
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, rl = lane & 15;
-  const int qstart = a.qstart[seq], base = h.ctx - h.qlen;
+  const int base = h.ctx - h.qlen;
   const int* bt = a.bt + (long)seq * a.max_blocks;
 
   const int row0 = blk * F::R;
@@ -505,7 +519,7 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
   }
 }
 
-// A workgroup's part of the list: run(sequence, its shape, kv head, row block, first key, last key, slot) for every piece of it.
+// A workgroup's part of the list: run(sequence, its first row, its shape, kv head, row block, first key, last key, slot) for every piece of it.
 template <class F> static __device__ __forceinline__ void walk(const TreeArgs& a, int R, F&& run) {
   const List q = scan_units(a, R);
   const bool lead = threadIdx.x == 0 && a.joins;
@@ -523,22 +537,23 @@ template <class F> static __device__ __forceinline__ void walk(const TreeArgs& a
   int u = me * part, start, slot = 2 * me;
   int seq = place_of(a, R, q, u, start);
   while (u < end) {
-    const Shape h = shape_of(a, seq, R);
+    const Shape h = shape_of(a, q, seq, R);
     const int n = uniform(a.nkv * h.nb * h.nt);
     if (u - start >= n) { ++seq; start += n; continue; }      // (units are left, so a sequence with units follows)
     const int nt = uniform(h.nt), nb = uniform(h.nb), row = uniform((u - start) / nt), range = u - start - row * nt;
     const int kvh = uniform(row / nb), blk = row - kvh * nb, take = min(nt - range, end - u);
     const int k0 = range * a.ulen, k1 = range + take == nt ? h.ctx : k0 + take * a.ulen;
+    const int qstart = qstart_of(a, q, seq);
     if (lead && range == 0 && take < nt) {
       int* to = a.joins + 8 * me;
       to[0] = slot;
       to[1] = (u + nt - 1) / part;
       to[2] = blk * R;
       to[3] = kvh;
-      to[4] = a.qstart[seq];
+      to[4] = qstart;
       to[5] = h.qlen;
     }
-    run(seq, h, kvh, blk, k0, k1, take == nt ? -1 : slot);
+    run(seq, qstart, h, kvh, blk, k0, k1, take == nt ? -1 : slot);
     slot = 2 * me + 1;
     u += take;
   }
@@ -547,8 +562,8 @@ template <class F> static __device__ __forceinline__ void walk(const TreeArgs& a
 template <int D, int RF, bool EIGHT>
 __global__ void __launch_bounds__(64 * NW, (RF > 1 || D > 64 ? 2 : EIGHT ? 3 : 4)) tree_attn_kernel(TreeArgs a) {
   __shared__ TreeSmem<D, RF, EIGHT> sm;
-  walk(a, Form<D, RF, EIGHT>::R, [&](int seq, const Shape& h, int kvh, int blk, int k0, int k1, int slot) __attribute__((always_inline)) {
-    piece<D, RF, EIGHT>(a, sm, seq, h, kvh, blk, k0, k1, slot);
+  walk(a, Form<D, RF, EIGHT>::R, [&](int seq, int qstart, const Shape& h, int kvh, int blk, int k0, int k1, int slot) __attribute__((always_inline)) {
+    piece<D, RF, EIGHT>(a, sm, seq, qstart, h, kvh, blk, k0, k1, slot);
   });
 }
 
@@ -571,13 +586,13 @@ template <int D, int RF> struct WideSmem {
 };
 
 template <int D, int RF>
-static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D, RF>& sm, const int seq, const Shape h, const int kvh, const int blk,
+static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D, RF>& sm, const int seq, const int qstart, const Shape h, const int kvh, const int blk,
                                                   const int k0, const int k1, const int slot) {
   using F = Wide<D, RF>;
   constexpr int CK = F::CK, KS = F::KS, NT = F::NT, KPG = F::KPG;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, rl = lane & 15;
-  const int qstart = a.qstart[seq], base = h.ctx - h.qlen, row0 = (blk * NW + wave) * 16 * RF;
+  const int base = h.ctx - h.qlen, row0 = (blk * NW + wave) * 16 * RF;
   const int* bt = a.bt + (long)seq * a.max_blocks;
   const bool idle = row0 >= h.qlen * a.G;                     // no row: this wave stages only
   const int steps = (k1 - k0 + CK - 1) / CK, last_block = (h.ctx - 1) >> 4;
@@ -734,8 +749,8 @@ static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D,
 
 template <int D, int RF> __global__ void __launch_bounds__(64 * NW, 2) tree_wide_kernel(TreeArgs a) {
   __shared__ WideSmem<D, RF> sm;
-  walk(a, Wide<D, RF>::R, [&](int seq, const Shape& h, int kvh, int blk, int k0, int k1, int slot) __attribute__((always_inline)) {
-    wide_piece<D, RF>(a, sm, seq, h, kvh, blk, k0, k1, slot);
+  walk(a, Wide<D, RF>::R, [&](int seq, int qstart, const Shape& h, int kvh, int blk, int k0, int k1, int slot) __attribute__((always_inline)) {
+    wide_piece<D, RF>(a, sm, seq, qstart, h, kvh, blk, k0, k1, slot);
   });
 }
 

@@ -1261,7 +1261,7 @@ def verify_drafts(target, tokens, uniform, seq_qstart, seq_qlen, max_nodes, pare
                     ok = real and u[q0 + i] * float(draft[q0 + i, x]) < px
                     w = p - draft[q0 + i].double()
                 else:
-                    ok = u[q0 + i] * mass < px
+                    ok = real and u[q0 + i] * max(mass, 0.0) < px
                     mass -= px
                     gone.add(x)
                 if ok:

@@ -11,20 +11,22 @@ constexpr int NTH = 256;
 
 // ------------------------------------------------------------------------------------------------ masks
 // Workgroup s < S: a node's word of ancestors (itself among them) and their number, from a walk up the parents in LDS; indices fall on the way,
-// so a word is whole when the walk leaves it.  Workgroups behind: rows that no sequence has become zero.
+// so a word is whole when the walk leaves it.  Workgroups behind: rows that no sequence has, or that lie past 32 W nodes of it, become zero.
 __global__ void __launch_bounds__(NTH) tree_mask_kernel(const int* __restrict__ parents, const int* __restrict__ qstart, const int* __restrict__ qlen,
                                                         int* __restrict__ mask, int* __restrict__ depth, int W, int S, int T) {
   __shared__ int par[MAX_NODES];
   if ((int)blockIdx.x >= S) {
     const int t = (blockIdx.x - S) * NTH + threadIdx.x;
     if (t >= T) return;
-    for (int s = 0; s < S; ++s)
-      if (t >= qstart[s] && t - qstart[s] < qlen[s]) return;
+    for (int s = 0; s < S; ++s) {
+      const int q0 = qstart[s], n = min(qlen[s], 32 * W);
+      if (t >= q0 && t - q0 < n && q0 >= 0 && q0 <= T - n) return;
+    }
     for (int w = 0; w < W; ++w) mask[(long)t * W + w] = 0;
     depth[t] = 0;
     return;
   }
-  const int q0 = qstart[blockIdx.x], n = min(qlen[blockIdx.x], min(32 * W, MAX_NODES));
+  const int q0 = qstart[blockIdx.x], n = min(qlen[blockIdx.x], 32 * W);
   if (q0 < 0 || q0 > T - n) return;
   for (int i = threadIdx.x; i < n; i += NTH) par[i] = parents[q0 + i];
   __syncthreads();

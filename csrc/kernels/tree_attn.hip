@@ -40,7 +40,8 @@ struct TreeArgs {
   float scale_log2;
 };
 
-// ---- the list of units (32-bit: the launcher makes units long enough)
+// ---- the list of units (32-bit: the launcher makes units long enough; lengths that contradict each other end at MOST and reach no memory but their own)
+constexpr int MOST = 1 << 30;
 struct Shape {
   int qlen, ctx, nb, nt;    // row blocks and key ranges
 };
@@ -57,10 +58,11 @@ static __device__ __forceinline__ Shape shape_of(const TreeArgs& a, int qlen, in
   Shape h;
   h.qlen = min(max(qlen, 0), a.T);
   h.ctx = min(max(ctx, 0), a.max_blocks * BS);
-  h.nb = (h.qlen * a.G + R - 1) / R;
+  h.nb = (h.qlen * a.G + R - 1) / R;                          // (T nq fits 32 bits)
   h.nt = a.ulen ? max(1, (h.ctx + a.ulen - 1) / a.ulen) : 1;
   return h;
 }
+static __device__ __forceinline__ int units_of(const TreeArgs& a, const Shape& h) { return (int)min((long)a.nkv * h.nb * h.nt, (long)MOST); }
 static __device__ __forceinline__ Shape shape_of(const TreeArgs& a, const List& q, int s, int R) {
   if (q.count == 1) return shape_of(a, __builtin_amdgcn_readlane(q.qlen, s), __builtin_amdgcn_readlane(q.ctx, s), R);
   return shape_of(a, a.qlen[s], a.ctx[s], R);
@@ -80,13 +82,13 @@ static __device__ __forceinline__ List scan_units(const TreeArgs& a, int R) {
     q.ctx = a.ctx[s];
     q.qstart = a.qstart[s];
     const Shape h = shape_of(a, q.qlen, q.ctx, R);
-    if (q.first + i < a.S) q.incl += a.nkv * h.nb * h.nt;
+    if (q.first + i < a.S) q.incl = min(q.incl + units_of(a, h), MOST);
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     if (o < a.S) {                                            // (lanes from S on only repeat the total)
       const int y = __shfl_up(q.incl, o, 64);
-      if (lane >= o) q.incl += y;
+      if (lane >= o) q.incl = min(q.incl + y, MOST);
     }
   }
   q.total = __builtin_amdgcn_readlane(q.incl, min(a.S, 64) - 1);
@@ -100,7 +102,7 @@ static __device__ __forceinline__ int place_of(const TreeArgs& a, int R, const L
   if (q.count == 1) return s;
   for (; s < a.S - 1; ++s) {
     const Shape h = shape_of(a, a.qlen[s], a.ctx[s], R);
-    const int n = uniform(a.nkv * h.nb * h.nt);
+    const int n = uniform(units_of(a, h));
     if (start + n > unit) break;
     start += n;
   }
@@ -538,8 +540,12 @@ template <class F> static __device__ __forceinline__ void walk(const TreeArgs& a
   int seq = place_of(a, R, q, u, start);
   while (u < end) {
     const Shape h = shape_of(a, q, seq, R);
-    const int n = uniform(a.nkv * h.nb * h.nt);
-    if (u - start >= n) { ++seq; start += n; continue; }      // (units are left, so a sequence with units follows)
+    const int n = uniform(units_of(a, h));
+    if (u - start >= n) {
+      if (++seq >= a.S) return;
+      start += n;
+      continue;
+    }
     const int nt = uniform(h.nt), nb = uniform(h.nb), row = uniform((u - start) / nt), range = u - start - row * nt;
     const int kvh = uniform(row / nb), blk = row - kvh * nb, take = min(nt - range, end - u);
     const int k0 = range * a.ulen, k1 = range + take == nt ? h.ctx : k0 + take * a.ulen;
@@ -547,7 +553,7 @@ template <class F> static __device__ __forceinline__ void walk(const TreeArgs& a
     if (lead && range == 0 && take < nt) {
       int* to = a.joins + 8 * me;
       to[0] = slot;
-      to[1] = (u + nt - 1) / part;
+      to[1] = min((u + nt - 1) / part, a.nwg - 1);
       to[2] = blk * R;
       to[3] = kvh;
       to[4] = qstart;
@@ -560,7 +566,7 @@ template <class F> static __device__ __forceinline__ void walk(const TreeArgs& a
 }
 
 template <int D, int RF, bool EIGHT>
-__global__ void __launch_bounds__(64 * NW, (RF > 1 || D > 64 ? 2 : EIGHT ? 3 : 4)) tree_attn_kernel(TreeArgs a) {
+__global__ void __launch_bounds__(64 * NW, (RF > 1 || D > 64 ? 2 : 3)) tree_attn_kernel(TreeArgs a) {
   __shared__ TreeSmem<D, RF, EIGHT> sm;
   walk(a, Form<D, RF, EIGHT>::R, [&](int seq, int qstart, const Shape& h, int kvh, int blk, int k0, int k1, int slot) __attribute__((always_inline)) {
     piece<D, RF, EIGHT>(a, sm, seq, qstart, h, kvh, blk, k0, k1, slot);
@@ -573,7 +579,7 @@ __global__ void __launch_bounds__(64 * NW, (RF > 1 || D > 64 ? 2 : EIGHT ? 3 : 4
 // rows: with rows of one wave only, every 48 read them again, and ragged trees of 80 to 160 rows (8 kv heads of 128, 32 sequences of 200 to 3000 keys)
 // ran at what L2 misses of four such readings allow.  (Loads straight to LDS made the compiler wait for all of them ahead of any LDS read.)
 template <int D, int RF> struct Wide {
-  static constexpr int CK = RF == 1 && D > 64 ? 32 : 64, KS = D / 32, NT = D / 16, TL = CK / 16, KPG = CK / 4, R = 16 * RF * NW;
+  static constexpr int CK = D > 64 ? 32 : 64, KS = D / 32, NT = D / 16, TL = CK / 16, KPG = CK / 4, R = 16 * RF * NW;
   // one-kilobyte slots of a stage: K a tile and 32 dims (slot t * KS + s), V eight keys a lane group and sixteen dims (KSL + e * NT + n)
   static constexpr int KSL = TL * KS, SL = KSL + NT * (CK / 32), GI = SL / NW, PAGES = 1024;
   static_assert(SL % NW == 0, "whole slots a wave");
@@ -699,14 +705,23 @@ static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D,
       f32x4 sc[RF][2];
 #pragma unroll
       for (int f = 0; f < RF; ++f) sc[f][0] = sc[f][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      // operands of a product are all on their way before its first instruction, V's while the weights are computed: read one by one, two waves a
+      // SIMD spent half their time waiting for LDS
+      bf16x8 kf[2][KS], vf[NT];
 #pragma unroll
       for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const bf16x8 kf = __builtin_bit_cast(bf16x8, ld16(ring + ((2 * e + t2) * KS + s) * 1024 + lane * 16));
+        for (int s = 0; s < KS; ++s) kf[t2][s] = __builtin_bit_cast(bf16x8, ld16(ring + ((2 * e + t2) * KS + s) * 1024 + lane * 16));
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int f = 0; f < RF; ++f) sc[f][t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[f][s], sc[f][t2], 0, 0, 0);
-        }
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int f = 0; f < RF; ++f)
+#pragma unroll
+          for (int t2 = 0; t2 < 2; ++t2) sc[f][t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t2][s], qf[f][s], sc[f][t2], 0, 0, 0);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) vf[n] = __builtin_bit_cast(bf16x8, ld16(ring + (F::KSL + e * NT + n) * 1024 + lane * 16));
+      __builtin_amdgcn_sched_barrier(0);
       bf16x8 pf[RF][1];
       if (!plain) {
 #pragma unroll
@@ -714,11 +729,9 @@ static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D,
       }
       weights<RF, NT, 2, false>(sc, nullptr, c, m, l, acc, pf);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const bf16x8 vf = __builtin_bit_cast(bf16x8, ld16(ring + (F::KSL + e * NT + n) * 1024 + lane * 16));
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int f = 0; f < RF; ++f) acc[f][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[f][0], acc[f][n], 0, 0, 0);
-      }
+        for (int f = 0; f < RF; ++f) acc[f][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[n], pf[f][0], acc[f][n], 0, 0, 0);
     }
     }
     if (i + 1 < steps) store(i + 1);

@@ -1190,7 +1190,8 @@ def tree_mask(parents, seq_qstart, seq_qlen, max_nodes):
     mask, depth = torch.zeros(T, W, dtype=torch.int64), torch.zeros(T, dtype=torch.int32)
     par = parents.tolist()
     for q0, n in zip(seq_qstart.tolist(), seq_qlen.tolist()):
-        for i in range(min(n, 32 * W, T - q0) if 0 <= q0 else 0):
+        n = min(n, 32 * W)
+        for i in range(n if 0 <= q0 <= T - n else 0):
             at, up = i, -1
             while at >= 0:
                 mask[q0 + i, at // 32] |= 1 << (at % 32)

@@ -105,6 +105,63 @@ def test_few_rows_of_short_contexts_in_one_launch(eight, seqs, d):
 
 
 @pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("qlen", [2, 4, 5, 8, 9, 16, 17])
+def test_row_blocks_of_every_form(eight, d, qlen):
+    """Twelve sequences of 900 keys, eight query heads to each of three: blocks of 16, 32 and 48 rows of a wave, of 64 and 128 of four, filled and a row over."""
+    s = step([(qlen, 900 + i) for i in range(11)] + [(1, 5)], 24, 3, d, eight, "tree", qlen)
+    near(attend(to(s, DEV), max_qlen=qlen, max_ctx=910), *attention64(s))
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("hints", [dict(max_qlen=1, max_ctx=1), dict(max_qlen=1), dict(max_ctx=16), dict(max_qlen=10 ** 6, max_ctx=10 ** 6)])
+def test_hints_that_are_wrong_cost_time_alone(eight, hints):
+    s = step([(40, 700), (9, 1300), (2, 2)], 8, 2, 64, eight, "tree", 15)
+    near(attend(to(s, DEV), **hints), *attention64(s))
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_contexts_shorter_than_their_new_tokens(eight):
+    """No key at all, or fewer than new tokens: rows ahead of the first key see nothing and are zero."""
+    s = step([(2, 0), (5, 3), (40, 7), (3, 50)], 4, 2, 64, eight, "chain", 16)
+    want, bound = attention64(s)
+    got = attend(to(s, DEV))
+    near(got, want, bound)
+    assert not got[:4].any() and not want[:4].any()
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+def test_other_scales(eight, scale):
+    """A negative scale turns the order of scores, 0 makes the mean.  Bounds as attention64's, whose scale is 1 / 8 here: queries carry the rest exactly
+    (-1.6 and 24 do not fit bf16: the expected value is computed with them in 64 bits)."""
+    s = step([(9, 300), (1, 40)], 4, 2, 64, eight, "tree", 17)
+    wide = dict(s, q=s["q"].double() * (8.0 * scale))
+    near(attend(to(s, DEV), scale=scale), *attention64(wide))
+
+
+def test_a_part_longer_than_its_window_of_pages():
+    """430 sequences over the same 20000 keys: a workgroup's part passes 16384 keys of one row block, so its pages are looked up again on the way."""
+    n, ctx, qlen, d = 430, 20000, 9, 64
+    s = to(step([(qlen, ctx)], 4, 1, d, False, "chain", 18), DEV)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    s["q"] = (1.5 * torch.randn(n * qlen, 4, d, device=DEV, generator=g)).bfloat16()
+    s["table"] = s["table"].repeat(n, 1)
+    s["qstart"], s["qlen"], s["ctx"] = i32(list(range(0, n * qlen, qlen)), DEV), i32([qlen] * n, DEV), i32([ctx] * n, DEV)
+    got = attend(s)
+    k, v = dense({t: None if x is None else x.cpu() for t, x in dict(s, table=s["table"][:1]).items()}, 0)
+    k, v = k[0].to(DEV), v[0].to(DEV)
+    see = torch.arange(ctx, device=DEV)[None] <= ctx - qlen + torch.arange(qlen, device=DEV)[:, None]
+    for b in range(0, n, 43):
+        x = s["q"][b * qlen:(b + 1) * qlen].double()                                        # [qlen, 4, d]
+        w = torch.softmax((x.transpose(0, 1) @ k.T / 8).masked_fill(~see, -math.inf), -1)   # [4, qlen, keys]
+        o, a = (w @ v).transpose(0, 1), (w @ v.abs()).transpose(0, 1)
+        ds = (d + 3) * 2.0 ** -24 * (x.abs() @ k.abs().T / 8).amax(-1)[..., None]
+        e = (2.0 ** -8 + 2 * ds + (2 * ctx + 16) * 2.0 ** -24) * a
+        near(got[b * qlen:(b + 1) * qlen], o.cpu(), (e + 2.0 ** -8 * (o.abs() + e)).cpu())
+
+
+@pytest.mark.parametrize("eight", [False, True])
 def test_rows_of_a_prompt_behind_a_cached_one(eight):
     s = step([(300, 300), (129, 1001)], 8, 2, 64, eight, "chain", 5)
     near(attend(to(s, DEV)), *attention64(s))
@@ -413,6 +470,15 @@ def test_masks(lens, most):
     start, n = i32([sum(lens[:i]) for i in range(len(lens))]), i32(lens)
     want, got = ref.tree_mask(par, start, n, most), ops.draft.tree_mask(par.to(DEV), start.to(DEV), n.to(DEV), most)
     assert torch.equal(want[0], got[0].cpu()) and torch.equal(want[1], got[1].cpu())
+
+
+def test_masks_of_sequences_that_do_not_fit():
+    """More nodes than max_nodes, a start outside the rows: those rows are zero."""
+    par = i32([-1] + list(range(69)) + [-1, 0, 0])
+    start, n = i32([0, 70, 500, -3]), i32([70, 3, 4, 2])
+    want, got = ref.tree_mask(par, start, n, 40), ops.draft.tree_mask(par.to(DEV), start.to(DEV), n.to(DEV), 40)
+    assert torch.equal(want[0], got[0].cpu()) and torch.equal(want[1], got[1].cpu())
+    assert not got[0][64:70].any() and bool(got[0][63].any())
 
 
 def test_no_sequences_and_no_rows():

@@ -577,7 +577,9 @@ __global__ void __launch_bounds__(64 * NW, (RF > 1 || D > 64 ? 2 : 3)) tree_attn
 // Four waves of 16 RF rows read every chunk from LDS, in two stages: a wave asks for its share of the next chunk, computes on this one and then writes
 // what has arrived.  One operand fragment is a kilobyte in lane order, read back as it lies, without conflicts.  K and V leave L2 once for 64 RF
 // rows: with rows of one wave only, every 48 read them again, and ragged trees of 80 to 160 rows (8 kv heads of 128, 32 sequences of 200 to 3000 keys)
-// ran at what L2 misses of four such readings allow.  (Loads straight to LDS made the compiler wait for all of them ahead of any LDS read.)
+// ran at what L2 misses of four such readings allow (115 us, 82 so).  512 rows of 8000 to 32000 keys: 203 us, 555 TFLOP/s; two waves a SIMD that wait for
+// the same chunk leave a quarter of the matrix cores' time used, and L2 misses of the row blocks take 5.2 TB/s.  (Loads straight to LDS made the compiler wait for all of
+// them ahead of any LDS read; 48 rows a wave spill, 64 keys a stage gain nothing.)
 template <int D, int RF> struct Wide {
   static constexpr int CK = D > 64 ? 32 : 64, KS = D / 32, NT = D / 16, TL = CK / 16, KPG = CK / 4, R = 16 * RF * NW;
   // one-kilobyte slots of a stage: K a tile and 32 dims (slot t * KS + s), V eight keys a lane group and sixteen dims (KSL + e * NT + n)

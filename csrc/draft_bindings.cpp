@@ -11,7 +11,7 @@
 
 extern "C" {
 int dllm_tree_attention(const void*, long, long, const void*, const void*, const float*, const float*, const int*, const int*, const int*, const int*,
-                        const int*, void*, float*, float*, int*, int, int, int, int, int, int, int, int, int, int, int, int, int, float, hipStream_t);
+                        const int*, void*, float*, float*, int*, int, int, int, int, int, int, int, int, int, int, int, int, int, int, int, float, hipStream_t);
 int dllm_tree_mask(const int*, const int*, const int*, int*, int*, int, int, int, hipStream_t);
 int dllm_verify_parts(int, int*);
 int dllm_verify(const void*, long, const void*, long, int, const int*, const int*, const float*, const int*, const int*, int*, int*, int*, double*, int*,
@@ -134,13 +134,17 @@ Tensor tree_attention(Tensor q, Tensor k, Tensor v, Tensor bt, Tensor qstart, Te
   int64_t nwg = (int64_t)cus(q) * 2 / 8 * 8;      // two workgroups a CU (three: 70 -> 81 us for single tokens over 8 bits)
   const int64_t R = 16 * rf * (wide ? 4 : 1);
   const int64_t blocks = S * c.nkv * ((most + R - 1) / R);      // row blocks, at most
-  // Keys of a unit: short ones share out short contexts evenly (1500 keys 49 us, 60 with 512), long ones leave fewer pieces to write and join
-  // (16000 keys, 96 rows 57 -> 45; 32000 keys of four sequences 191 -> 180).  What one unit holds is not split: one launch.
-  int64_t ulen = keys > 4096 ? 512 : keys > 256 ? 256 : 0;
+  // Keys of a unit (of whole rounds of a workgroup's chunks), units that a row block's way in and out counts for, and units of a part, at least: short
+  // parts of long contexts leave many pieces to join.  us with a way of 0 / 2 / 3 / 4 / 6 units: ragged trees of 80 to 160 rows 94 / 78 / 75 / 74 / 75, 160
+  // rows of a chain 108 / 91 / 87 / 86 / 92; 48 rows over e4m3 39 / 37 / 35 / 35 / 36; 16 rows are bound by memory, 64 single tokens 113 / 116 / 118.
+  // With units of 256 keys and no way 82, 100, 37, 113.  Parts of 512 keys and more from 4096 on: one sequence of 16000 65 -> 55.  A context of up to
+  // 256 keys is one unit, not split: one launch.
+  int64_t ulen = keys <= 256 ? 0 : wide ? 64 : c.eight && rf == 1 ? 256 : 128;
+  const int64_t way = wide ? 4 : rf > 1 ? 3 : c.eight ? 1 : 0, least = ulen ? (keys > 4096 ? 512 : 256) / ulen : 1;
   // the list of units is counted in 32 bits
   const int64_t listed = c.nkv * (T * G / R + S);
   NEED(T * nq <= 0x7fffffff && listed < (1 << 30), "tree_attention: too many");
-  while (ulen && listed * (max_blocks * BS / ulen + 1) >= (1 << 30)) ulen *= 2;
+  while (ulen && listed * (max_blocks * BS / ulen + 1 + way) >= (1 << 30)) ulen *= 2;
   nwg = std::min(nwg, (blocks * (ulen ? (keys + ulen - 1) / ulen : 1) + 7) / 8 * 8);
   Tensor part;
   float *po = nullptr, *pml = nullptr;
@@ -156,7 +160,7 @@ Tensor tree_attention(Tensor q, Tensor k, Tensor v, Tensor bt, Tensor qstart, Te
   launched(dllm_tree_attention(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), ks ? ks->data_ptr<float>() : nullptr,
                                vs ? vs->data_ptr<float>() : nullptr, bt.data_ptr<int>(), qstart.data_ptr<int>(), qlen.data_ptr<int>(), ctx.data_ptr<int>(),
                                mask ? mask->data_ptr<int>() : nullptr, o.data_ptr(), po, pml, joins, (int)W, (int)S, (int)T, (int)nq, (int)c.nkv, (int)d,
-                               (int)max_blocks, (int)c.blocks, (int)nwg, (int)ulen, rf, wide, (int)join_rows, (float)scale, stream()),
+                               (int)max_blocks, (int)c.blocks, (int)nwg, (int)ulen, (int)way, (int)least, rf, wide, (int)join_rows, (float)scale, stream()),
            "tree_attention");
   return o;
 }

@@ -16,7 +16,7 @@
 // ahead of the weight's rounding to bf16; the sum of weights is of the unrounded ones.
 //
 // Split: all (sequence, kv head, row block, range of `ulen` keys) form one list, cut into equal parts for the workgroups that fit the chip at
-// once; every workgroup finds its part from the lengths on the device, so ragged batches are even, nothing is planned on the host and a
+// once; a row block counts for some units more than its keys, for the way in and out of it (queries, masks, sums).  Every workgroup finds its part from the lengths on the device, so ragged batches are even, nothing is planned on the host and a
 // captured graph takes new lengths.  A part's first and last piece may be of a row block that others hold too: their sums go to the workspace
 // in 32 bits and a second launch joins them, in order (no atomics: the same bits every time).
 #include "common.h"
@@ -36,14 +36,14 @@ struct TreeArgs {
   u16* out;                 // [T, nq, d]
   float *part_o, *part_ml;  // [2 nwg, R, d], [2 nwg, R, 2]
   int* joins;               // [nwg, 8]: what the join has to do for a part that begins a block others end; [nwg]: the number of parts
-  int W, S, T, nq, nkv, G, max_blocks, num_blocks, nwg, ulen;
+  int W, S, T, nq, nkv, G, max_blocks, num_blocks, nwg, ulen, way, least;
   float scale_log2;
 };
 
 // ---- the list of units (32-bit: the launcher makes units long enough; lengths that contradict each other end at MOST and reach no memory but their own)
 constexpr int MOST = 1 << 30;
 struct Shape {
-  int qlen, ctx, nb, nt;    // row blocks and key ranges
+  int qlen, ctx, nb, nt;    // row blocks, and units of each: a.way for its way in and out, and its key ranges
 };
 
 static __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -59,7 +59,7 @@ static __device__ __forceinline__ Shape shape_of(const TreeArgs& a, int qlen, in
   h.qlen = min(max(qlen, 0), a.T);
   h.ctx = min(max(ctx, 0), a.max_blocks * BS);
   h.nb = (h.qlen * a.G + R - 1) / R;                          // (T nq fits 32 bits)
-  h.nt = a.ulen ? max(1, (h.ctx + a.ulen - 1) / a.ulen) : 1;
+  h.nt = a.ulen ? a.way + max(1, (h.ctx + a.ulen - 1) / a.ulen) : 1;
   return h;
 }
 static __device__ __forceinline__ int units_of(const TreeArgs& a, const Shape& h) { return (int)min((long)a.nkv * h.nb * h.nt, (long)MOST); }
@@ -86,7 +86,7 @@ static __device__ __forceinline__ List scan_units(const TreeArgs& a, int R) {
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    if (o < a.S) {                                            // (lanes from S on only repeat the total)
+    if (o < a.S) {                                            // (lanes from S on are not looked at)
       const int y = __shfl_up(q.incl, o, 64);
       if (lane >= o) q.incl = min(q.incl + y, MOST);
     }
@@ -108,7 +108,7 @@ static __device__ __forceinline__ int place_of(const TreeArgs& a, int R, const L
   }
   return s;
 }
-static __device__ __forceinline__ int part_len(const TreeArgs& a, int total) { return uniform((total + a.nwg - 1) / a.nwg); }
+static __device__ __forceinline__ int part_len(const TreeArgs& a, int total) { return max(uniform((total + a.nwg - 1) / a.nwg), a.least); }
 
 // ---- operands
 static __device__ __forceinline__ uint4 flip(uint4 v, uint32_t sign) { return make_uint4(v.x ^ sign, v.y ^ sign, v.z ^ sign, v.w ^ sign); }
@@ -537,30 +537,33 @@ template <class F> static __device__ __forceinline__ void walk(const TreeArgs& a
   if (lead && me == 0) a.joins[8 * a.nwg] = parts;
   if (lead) a.joins[8 * me] = -1;
   int u = me * part, start, slot = 2 * me;
-  int seq = place_of(a, R, q, u, start);
+  int seq = place_of(a, R, q, u, start), qstart = qstart_of(a, q, seq);
+  Shape h = shape_of(a, q, seq, R);                           // (later ones from memory: the lanes' lengths are not kept for them)
   while (u < end) {
-    const Shape h = shape_of(a, q, seq, R);
     const int n = uniform(units_of(a, h));
     if (u - start >= n) {
       if (++seq >= a.S) return;
       start += n;
+      h = shape_of(a, a.qlen[seq], a.ctx[seq], R);
+      qstart = a.qstart[seq];
       continue;
     }
-    const int nt = uniform(h.nt), nb = uniform(h.nb), row = uniform((u - start) / nt), range = u - start - row * nt;
-    const int kvh = uniform(row / nb), blk = row - kvh * nb, take = min(nt - range, end - u);
-    const int k0 = range * a.ulen, k1 = range + take == nt ? h.ctx : k0 + take * a.ulen;
-    const int qstart = qstart_of(a, q, seq);
-    if (lead && range == 0 && take < nt) {
-      int* to = a.joins + 8 * me;
-      to[0] = slot;
-      to[1] = min((u + nt - 1) / part, a.nwg - 1);
-      to[2] = blk * R;
-      to[3] = kvh;
-      to[4] = qstart;
-      to[5] = h.qlen;
+    const int nt = uniform(h.nt), nb = uniform(h.nb), row = uniform((u - start) / nt), at = u - start - row * nt, take = min(nt - at, end - u);
+    const int kvh = uniform(row / nb), blk = row - kvh * nb, r0 = max(at - a.way, 0), r1 = at + take - a.way, ranges = nt - a.way;
+    if (r1 > r0) {
+      const bool whole = r0 == 0 && r1 == ranges;
+      if (lead && r0 == 0 && !whole) {
+        int* to = a.joins + 8 * me;
+        to[0] = slot;
+        to[1] = min((u - at + nt - 1) / part, a.nwg - 1);
+        to[2] = blk * R;
+        to[3] = kvh;
+        to[4] = qstart;
+        to[5] = h.qlen;
+      }
+      run(seq, qstart, h, kvh, blk, r0 * a.ulen, r1 == ranges ? h.ctx : r1 * a.ulen, whole ? -1 : slot);
+      slot = 2 * me + 1;
     }
-    run(seq, qstart, h, kvh, blk, k0, k1, take == nt ? -1 : slot);
-    slot = 2 * me + 1;
     u += take;
   }
 }
@@ -639,14 +642,10 @@ static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D,
   }
 
   uint4 next[F::GI];                                          // this wave's share of a chunk
-  int next_real = 0;                                          // keys of this lane's that exist
-  bool next_plain = false;
   auto load = [&](int i) {
     const int kb = k0 + CK * i, at = (kb >> 4) - first;
     const int pk = sm.page[at + (CK == 64 ? rl >> 2 : rl >> 3)], pv = sm.page[at + (CK == 64 ? g : g >> 1)];
     const long hk = ((long)max(pk, 0) * a.nkv + kvh) * BS + (CK == 64 ? 0 : 8 * ((rl >> 2) & 1)) + (rl & 3), hv = ((long)max(pv, 0) * a.nkv + kvh) * BS;
-    next_plain = kb + CK <= base && !__any(pv < 0);
-    next_real = pv >= 0 ? h.ctx - kb - KPG * g : 0;
 #pragma unroll
     for (int j = 0; j < F::GI; ++j) {
       const int p = wave * F::GI + j;                         // uniform
@@ -662,8 +661,10 @@ static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D,
   };
   auto store = [&](int i) {
     unsigned char* ring = sm.ring[i & 1];
-    bool odd = false;
-    if (!next_plain) {
+    const int kb = k0 + CK * i, pv = sm.page[(kb >> 4) - first + (CK == 64 ? g : g >> 1)];
+    if (kb + CK > base || __any(pv < 0)) {
+      const int n = pv >= 0 ? h.ctx - kb - KPG * g : 0;       // keys of this lane's that exist
+      bool odd = false;
       // what no row may see (keys past ctx, pages outside the pool: stale memory) is zero in V; an infinity or NaN of a drafted token that a
       // row does not see would reach it as 0 * inf, so those are zero too and added at the end, to the rows that see them
 #pragma unroll
@@ -673,7 +674,7 @@ static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D,
         uint32_t w[4] = {next[j].x, next[j].y, next[j].z, next[j].w};
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int left = min(max(next_real - 8 * (v / NT) - 2 * x, 0), 2);
+          const int left = min(max(n - 8 * (v / NT) - 2 * x, 0), 2);
           w[x] &= left == 2 ? ~0u : (1u << (16 * left)) - 1u;
           odd |= odd_bits<false>(w[x]) != 0;
           w[x] = tame<false>(w[x]);
@@ -821,17 +822,17 @@ template <int D> int launch_d(const TreeArgs& a, int rf, bool wide, int rows, hi
 }
 }  // namespace
 
-// rf: a wave has 16 rf rows (bf16 1 or 2, e4m3 up to 3).  wide (bf16): a row block is four waves' rows, else one's.  ulen: keys of a unit, a multiple of 256; 0: a row block is
-// one unit (no workspace, one launch).  rows: those of a block that the join's grid has waves for.
+// rf: a wave has 16 rf rows (bf16 1 or 2, e4m3 up to 3).  wide (bf16): a row block is four waves' rows, else one's.  ulen: keys of a unit, a multiple of 64; 0: a row block is
+// one unit (no workspace, one launch).  way: units that a row block counts for beside its keys; least: units of a part.  rows: those of a block that the join's grid has waves for.
 extern "C" int dllm_tree_attention(const void* q, long q_ts, long q_hs, const void* kc, const void* vc, const float* ks, const float* vs,
                                    const int* bt, const int* qstart, const int* qlen, const int* ctx, const int* mask, void* out, float* part_o,
-                                   float* part_ml, int* joins, int W, int S, int T, int nq, int nkv, int d, int max_blocks, int num_blocks, int nwg, int ulen,
+                                   float* part_ml, int* joins, int W, int S, int T, int nq, int nkv, int d, int max_blocks, int num_blocks, int nwg, int ulen, int way, int least,
                                    int rf, int wide, int rows, float scale, hipStream_t st) {
   if (nkv < 1 || nq < nkv || nq % nkv || rf < 1 || rf > 3 || rows < 1) return -1;
   if ((ks == nullptr) != (vs == nullptr) || S < 1 || T < 1 || max_blocks < 1 || num_blocks < 1 || nwg < 1) return -2;
-  if (ulen < 0 || ulen % 256 || (ulen && (!part_o || !part_ml || !joins))) return -3;
+  if (ulen < 0 || ulen % 64 || way < 0 || least < 1 || (ulen && (!part_o || !part_ml || !joins))) return -3;
   TreeArgs a{(const u16*)q, q_ts, q_hs, kc, vc, ks, vs, bt, qstart, qlen, ctx, mask, (u16*)out, part_o, part_ml,
-             ulen ? joins : nullptr, W, S, T, nq, nkv, nq / nkv, max_blocks, num_blocks, nwg, ulen, scale * LOG2E};
+             ulen ? joins : nullptr, W, S, T, nq, nkv, nq / nkv, max_blocks, num_blocks, nwg, ulen, ulen ? way : 0, ulen ? least : 1, scale * LOG2E};
   switch (d) {
     case 64: return launch_d<64>(a, rf, wide, rows, st);
     case 96: return launch_d<96>(a, rf, wide, rows, st);

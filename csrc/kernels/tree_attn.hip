@@ -775,10 +775,9 @@ template <int D, int RF> __global__ void __launch_bounds__(64 * NW, 2) tree_wide
 template <int D>
 __global__ void __launch_bounds__(64 * NW) tree_join_kernel(TreeArgs a, int R) {
   const int i0 = blockIdx.x;
-  if (i0 >= a.joins[8 * a.nwg]) return;
   const int* to_do = a.joins + 8 * i0;
-  const int first = to_do[0], i1 = to_do[1], row0 = to_do[2], kvh = to_do[3], qstart = to_do[4], qlen = to_do[5];
-  if (first < 0) return;
+  const int parts = a.joins[8 * a.nwg], first = to_do[0], i1 = to_do[1], row0 = to_do[2], kvh = to_do[3], qstart = to_do[4], qlen = to_do[5];
+  if (i0 >= parts || first < 0) return;                       // (asked for together: a trip to memory less)
   constexpr int LR = D / 4 <= 16 ? 16 : 32, RW = 64 * NW / LR;      // lanes of a row (four values each), rows at a time
   const int lr = threadIdx.x % LR, col = min(4 * lr, D - 4);
   for (int rr = RW * blockIdx.y + threadIdx.x / LR; rr < R; rr += RW * gridDim.y) {
@@ -788,16 +787,29 @@ __global__ void __launch_bounds__(64 * NW) tree_join_kernel(TreeArgs a, int R) {
     auto slot_row = [&](int i) { return (long)(i == i0 ? first : 2 * i) * R + rr; };
     float M = -INFINITY, L = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int i = i0; i <= i1; ++i) M = fmaxf(M, a.part_ml[2 * slot_row(i)]);
-    const float Ms = M == -INFINITY ? 0.f : M;
-#pragma unroll 4
-    for (int i = i0; i <= i1; ++i) {
-      const long at = slot_row(i);
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
-      const float w = __builtin_amdgcn_exp2f(ml.x - Ms);
-      L += ml.y * w;
-      o += *reinterpret_cast<const f32x4*>(a.part_o + at * D + col) * w;
+    for (int i = i0; i <= i1; i += 4) {                       // four pieces' sums and maxima in one trip
+      float2 ml[4];
+      f32x4 x[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const long at = slot_row(min(i + c, i1));
+        ml[c] = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+        x[c] = *reinterpret_cast<const f32x4*>(a.part_o + at * D + col);
+      }
+      float top = M;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) top = fmaxf(top, ml[c].x);
+      const float ts = top == -INFINITY ? 0.f : top, w0 = __builtin_amdgcn_exp2f(M - ts);
+      M = top;
+      L *= w0;
+      o *= w0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (i + c > i1) continue;
+        const float w = __builtin_amdgcn_exp2f(ml[c].x - ts);
+        L += ml[c].y * w;
+        o += x[c] * w;
+      }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     if (4 * lr < D)

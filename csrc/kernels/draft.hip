@@ -88,7 +88,7 @@ struct VerifySmem {
   int par[MAX_NODES], tok[MAX_NODES], nxt[MAX_NODES], out[MAX_NODES];
   double px[MAX_NODES];
   unsigned char ok[MAX_NODES];
-  double wsum[NTH / 64][2], base;
+  double wsum[NTH / 64][2];
   int wlast[NTH / 64][2];
   int nout;
 };
@@ -323,7 +323,6 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_walk_kernel(Ver
 template <class T> __global__ void __launch_bounds__(NTH) verify_pick_kernel(VerifyArgs a) {
   __shared__ VerifySmem sm;
   __shared__ double cum[NTH];
-  __shared__ int pick;
   const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int* f = a.found + ((long)s * (a.P + 1) + a.P) * 2;
   const int last = f[0];
@@ -353,6 +352,16 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_pick_kernel(Ver
     __syncthreads();
     return x;
   };
+  // The first thread whose sum passes t, NTH if none does (not the one between two sums: rounding may leave sums of neighbours in the wrong order).
+  auto first_over = [&](double sum, double t) {
+    const unsigned long long over = __ballot(sum > t);
+    if (lane == 0) sm.wlast[wid][1] = over ? 64 * wid + __builtin_ctzll(over) : NTH;
+    __syncthreads();
+    int m = NTH;
+#pragma unroll
+    for (int i = 0; i < NTH / 64; ++i) m = min(m, sm.wlast[i][1]);
+    return m;
+  };
   int which = 0;
   const double mine = tid < a.P ? sums[2 * tid] : 0.0, own_p = tid < a.P ? sums[2 * tid + 1] : 0.0;
   const int last_w = tid < a.P ? lasts[2 * tid] : -1, last_p = tid < a.P ? lasts[2 * tid + 1] : -1;
@@ -367,12 +376,8 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_pick_kernel(Ver
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) l = max(l, __shfl_xor(l, o, 64));
   if (lane == 0) sm.wlast[wid][0] = l;
-  if (tid == 0) pick = -1;
-  __syncthreads();
-  if (incl > t && (tid == 0 || !(cum[tid - 1] > t))) { pick = tid; sm.base = tid ? cum[tid - 1] : 0.0; }
-  __syncthreads();
-  const int part = pick;
-  if (part < 0) {                                                    // (infinite sums, or u = 1)
+  const int part = first_over(incl, t);
+  if (part >= a.P) {                                                 // (infinite sums, or u = 1)
     if (tid == 0) {
       int m = -1;
       for (int i = 0; i < NTH / 64; ++i) m = max(m, sm.wlast[i][0]);
@@ -380,7 +385,7 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_pick_kernel(Ver
     }
     return;
   }
-  const double base = sm.base;
+  const double base = part ? cum[part - 1] : 0.0;
   const int v0 = part * a.part, v1 = min(a.V, v0 + a.part), each = a.part / NTH;
   left_out(a, sm, which ? 0 : n, last, v0, v1);
   const T* p = (const T*)a.target + (long)(q0 + last) * a.target_ld;
@@ -403,9 +408,9 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_pick_kernel(Ver
     own += x[0]; own += x[1]; own += x[2]; own += x[3];
   }
   const double up = base + scan(own), down = tid ? base + cum[tid - 1] : base;
-  if (tid == 0) pick = -1;
-  __syncthreads();
-  if (up > t && !(down > t)) {
+  const int who = first_over(up, t);
+  if (who == NTH && tid == 0) a.next[s] = max(lasts[2 * part + which], 0);
+  if (tid == who) {
     double run = down;
     int got = -1;
 #pragma unroll
@@ -419,10 +424,8 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_pick_kernel(Ver
       for (int j = 0; j < 4; ++j)
         if (x[j] > 0.0 && !(run > t)) { run += x[j]; got = v + j; }
     }
-    pick = got;
+    a.next[s] = got >= 0 ? got : max(lasts[2 * part + which], 0);
   }
-  __syncthreads();
-  if (tid == 0) a.next[s] = pick >= 0 ? pick : max(lasts[2 * part + which], 0);
 }
 
 // ------------------------------------------------------------------------------------------------ keep

@@ -267,7 +267,7 @@ static __device__ __forceinline__ void add_odd(const TreeArgs& a, const int* bt,
 // Where a piece goes: the output, or slot `slot` of the workspace (< 0: the output).
 template <int D, int RF, bool EIGHT>
 static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, EIGHT>& sm, const int seq, const int qstart, const Shape h, const int kvh, const int blk,
-                                             const int k0, const int k1, const int slot) {
+                                             const int k0, const int k1, const int turn, const int slot) {
   using F = Form<D, RF, EIGHT>;
   constexpr int CK = F::CK, KS = F::KS, NT = F::NT, TL = F::TL, KPG = F::KPG;
   constexpr int KW = EIGHT ? 2 : 4, VW = EIGHT && CK == 32 ? 2 : 4;     // words of a lane's K step and V row
@@ -371,8 +371,11 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
 
   // K of the next chunk is asked for as soon as the scores have used this one's registers, V as soon as the second product has, pages a chunk
   // ahead of both: two chunks' latencies overlap without registers for two chunks.
-  int kb = k0 + CK * wave;
-  if (kb < k1) pages(kb, pk, pv);
+  constexpr int ROUND = CK * NW;
+  const int k_wave = k0 + CK * wave;
+  int left = (k1 - k_wave + ROUND - 1) / ROUND, kb = k_wave + turn < k1 ? k_wave + turn : k_wave;
+  auto after = [&](int x) { return x + ROUND < k1 ? x + ROUND : k_wave; };
+  if (left > 0) pages(kb, pk, pv);
   if constexpr (F::QL) {
 #pragma unroll
     for (int f = 0; f < RF; ++f)
@@ -386,10 +389,10 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
 #pragma unroll
       for (int s = 0; s < KS; ++s) qr[f][s] = __builtin_bit_cast(bf16x8, q_at(f, s));
   }
-  if (kb < k1) {
+  if (left > 0) {
     load_k(pk);
     load_v(kb, pv);
-    pages(kb + CK * NW, pk_n, pv_n);
+    pages(after(kb), pk_n, pv_n);
   }
   __syncthreads();                                            // the piece before is done with LDS
   if (threadIdx.x == 0) sm.odd = 0;
@@ -402,8 +405,9 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
       }
   }
   __syncthreads();
-  for (int next; kb < k1; kb = next) {
-    next = kb + CK * NW;
+  for (int next; left > 0; kb = next) {
+    next = after(kb);
+    --left;
     const bool paged = in_pool(pv);
     const bool plain = kb + CK <= base && !__any(!paged);     // every row sees the whole chunk
     bool odd = false;
@@ -434,7 +438,7 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
         for (int t = 0; t < TL; ++t) sc[f][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t], qf, sc[f][t], 0, 0, 0);
       }
     }
-    if (next < k1) load_k(pk_n);
+    if (left > 0) load_k(pk_n);
     bf16x8 pf[RF][TL / 2];
     scale_scores<RF, TL, EIGHT>(sc, ks);
     if (!plain) {
@@ -473,10 +477,10 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
         for (int f = 0; f < RF; ++f) acc[f][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[f][e], acc[f][n], 0, 0, 0);
       }
     if constexpr (EIGHT) __builtin_amdgcn_wave_barrier();     // scales are read before the next chunk's are written
-    if (next < k1) {
+    if (left > 0) {
       load_v(next, pv_n);
       pv = pv_n;
-      pages(next + CK * NW, pk_n, pv_n);
+      pages(after(next), pk_n, pv_n);
     }
   }
 
@@ -521,7 +525,9 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
   }
 }
 
-// A workgroup's part of the list: run(sequence, its first row, its shape, kv head, row block, first key, last key, slot) for every piece of it.
+// A workgroup's part of the list: run(sequence, its first row, its shape, kv head, row block, first key, last key, turn, slot) for every piece of it.
+// A piece begins `turn` keys behind its first one and comes to those in the end: parts of the row blocks of a kv head, which read the same keys and are cut at
+// different ones, are so at the same keys (modulo a part) at the same time, and find them in L2.
 template <class F> static __device__ __forceinline__ void walk(const TreeArgs& a, int R, F&& run) {
   const List q = scan_units(a, R);
   const bool lead = threadIdx.x == 0 && a.joins;
@@ -561,7 +567,8 @@ template <class F> static __device__ __forceinline__ void walk(const TreeArgs& a
         to[4] = qstart;
         to[5] = h.qlen;
       }
-      run(seq, qstart, h, kvh, blk, r0 * a.ulen, r1 == ranges ? h.ctx : r1 * a.ulen, whole ? -1 : slot);
+      const int past = r0 % part, turn = past && part - past < r1 - r0 ? part - past : 0;
+      run(seq, qstart, h, kvh, blk, r0 * a.ulen, r1 == ranges ? h.ctx : r1 * a.ulen, turn * a.ulen, whole ? -1 : slot);
       slot = 2 * me + 1;
     }
     u += take;
@@ -571,8 +578,8 @@ template <class F> static __device__ __forceinline__ void walk(const TreeArgs& a
 template <int D, int RF, bool EIGHT>
 __global__ void __launch_bounds__(64 * NW, (RF > 1 || D > 64 ? 2 : 3)) tree_attn_kernel(TreeArgs a) {
   __shared__ TreeSmem<D, RF, EIGHT> sm;
-  walk(a, Form<D, RF, EIGHT>::R, [&](int seq, int qstart, const Shape& h, int kvh, int blk, int k0, int k1, int slot) __attribute__((always_inline)) {
-    piece<D, RF, EIGHT>(a, sm, seq, qstart, h, kvh, blk, k0, k1, slot);
+  walk(a, Form<D, RF, EIGHT>::R, [&](int seq, int qstart, const Shape& h, int kvh, int blk, int k0, int k1, int turn, int slot) __attribute__((always_inline)) {
+    piece<D, RF, EIGHT>(a, sm, seq, qstart, h, kvh, blk, k0, k1, turn, slot);
   });
 }
 
@@ -587,18 +594,20 @@ template <int D, int RF> struct Wide {
   static constexpr int CK = D > 64 ? 32 : 64, KS = D / 32, NT = D / 16, TL = CK / 16, KPG = CK / 4, R = 16 * RF * NW;
   // one-kilobyte slots of a stage: K a tile and 32 dims (slot t * KS + s), V eight keys a lane group and sixteen dims (KSL + e * NT + n)
   static constexpr int KSL = TL * KS, SL = KSL + NT * (CK / 32), GI = SL / NW, PAGES = 1024;
-  static_assert(SL % NW == 0, "whole slots a wave");
+  // waves 0 and 1 stage K, 2 and 3 V, whole rows of tiles each
+  static_assert(SL == NW * GI && KSL == 2 * GI && GI % KS == 0 && NT % GI == 0, "a wave's slots");
 };
 template <int D, int RF> struct WideSmem {
   using F = Wide<D, RF>;
   alignas(16) unsigned char ring[2][F::SL * 1024];
   int page[F::PAGES];                                         // from block `first` of the sequence on; -1: outside the pool
   int odd;                                                    // infinities or NaN among V were left out
+  int holes;                                                  // a page outside the pool was met
 };
 
 template <int D, int RF>
 static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D, RF>& sm, const int seq, const int qstart, const Shape h, const int kvh, const int blk,
-                                                  const int k0, const int k1, const int slot) {
+                                                  const int k0, const int k1, const int turn, const int slot) {
   using F = Wide<D, RF>;
   constexpr int CK = F::CK, KS = F::KS, NT = F::NT, KPG = F::KPG;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -618,18 +627,21 @@ static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D,
     for (int s = 0; s < KS; ++s)
       qf[f][s] = __builtin_bit_cast(bf16x8, real(t) ? flip(ld16(a.q + (qstart + (long)t) * a.q_ts + head * a.q_hs + 32 * s + 8 * g), sign) : make_uint4(0u, 0u, 0u, 0u));
   }
-  int first = k0 >> 4;
+  int first = k0 >> 4, holes;
   auto fill = [&](int from) {
     first = from;
     for (int i = threadIdx.x; i < F::PAGES; i += 64 * NW) {
       const int b = from + i, p = b <= last_block ? bt[b] : -1;
-      sm.page[i] = (unsigned)p < (unsigned)a.num_blocks ? p : -1;
+      const bool in = (unsigned)p < (unsigned)a.num_blocks;
+      sm.page[i] = in ? p : -1;
+      if (b <= last_block && !in) sm.holes = 1;
     }
+    __syncthreads();
+    holes = uniform(sm.holes);
   };
   __syncthreads();                                            // the piece before is done with LDS
   if (threadIdx.x == 0) sm.odd = 0;
   fill(first);
-  __syncthreads();
 
   f32x4 acc[RF][NT];
   float m[RF], l[RF];
@@ -642,39 +654,36 @@ static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D,
   }
 
   uint4 next[F::GI];                                          // this wave's share of a chunk
+  const int rot = steps * CK <= BS * F::PAGES ? turn / CK : 0;
+  auto key_of = [&](int i) { return k0 + CK * (i + rot < steps ? i + rot : i + rot - steps); };
+  const bool of_k = wave < NW / 2;
+  const int own = (wave % (NW / 2)) * F::GI;                  // the first of its slots, of K's or of V's
+  const int from = of_k ? ((CK == 64 ? 0 : 8 * ((rl >> 2) & 1)) + 4 * (own / KS) + (rl & 3)) * D + 8 * g
+                        : (16 * (own % NT) + rl) * BS + (CK == 64 ? 8 * (own / NT) : 8 * (g & 1));
+  const u16* lane_src = (const u16*)(of_k ? a.kc : a.vc) + (long)kvh * BS * D + from;
+  const int lane_page = CK == 64 ? (of_k ? rl >> 2 : g) : (of_k ? rl >> 3 : g >> 1);
+  const uint32_t page_len = (uint32_t)a.nkv * BS * D;         // (the launcher: fewer than 2^16 kv heads)
+  int page = 0;
   auto load = [&](int i) {
-    const int kb = k0 + CK * i, at = (kb >> 4) - first;
-    const int pk = sm.page[at + (CK == 64 ? rl >> 2 : rl >> 3)], pv = sm.page[at + (CK == 64 ? g : g >> 1)];
-    const long hk = ((long)max(pk, 0) * a.nkv + kvh) * BS + (CK == 64 ? 0 : 8 * ((rl >> 2) & 1)) + (rl & 3), hv = ((long)max(pv, 0) * a.nkv + kvh) * BS;
+    page = sm.page[(key_of(i) >> 4) - first + lane_page];
+    const u16* x = lane_src + (uint64_t)(uint32_t)max(page, 0) * page_len;
 #pragma unroll
-    for (int j = 0; j < F::GI; ++j) {
-      const int p = wave * F::GI + j;                         // uniform
-      const u16* src;
-      if (p < F::KSL) {
-        src = (const u16*)a.kc + (hk + 4 * (p / KS)) * D + 32 * (p % KS) + 8 * g;
-      } else {
-        const int v = p - F::KSL, n = v % NT, e = v / NT;
-        src = (const u16*)a.vc + (hv * D + (16 * n + rl) * BS) + (CK == 64 ? 8 * e : 8 * (g & 1));
-      }
-      next[j] = ld16(src);
-    }
+    for (int j = 0; j < F::GI; ++j) next[j] = ld16(x + (of_k ? 4 * (j / KS) * D + 32 * (j % KS) : 16 * j * BS));
   };
   auto store = [&](int i) {
     unsigned char* ring = sm.ring[i & 1];
-    const int kb = k0 + CK * i, pv = sm.page[(kb >> 4) - first + (CK == 64 ? g : g >> 1)];
-    if (kb + CK > base || __any(pv < 0)) {
-      const int n = pv >= 0 ? h.ctx - kb - KPG * g : 0;       // keys of this lane's that exist
+    const int kb = key_of(i);
+    if (!of_k && (kb + CK > base || holes)) {
+      const int n = page >= 0 ? h.ctx - kb - KPG * g : 0;     // keys of this lane's that exist
       bool odd = false;
       // what no row may see (keys past ctx, pages outside the pool: stale memory) is zero in V; an infinity or NaN of a drafted token that a
       // row does not see would reach it as 0 * inf, so those are zero too and added at the end, to the rows that see them
 #pragma unroll
       for (int j = 0; j < F::GI; ++j) {
-        const int v = wave * F::GI + j - F::KSL;
-        if (v < 0) continue;
         uint32_t w[4] = {next[j].x, next[j].y, next[j].z, next[j].w};
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int left = min(max(n - 8 * (v / NT) - 2 * x, 0), 2);
+          const int left = min(max(n - 8 * (own / NT) - 2 * x, 0), 2);
           w[x] &= left == 2 ? ~0u : (1u << (16 * left)) - 1u;
           odd |= odd_bits<false>(w[x]) != 0;
           w[x] = tame<false>(w[x]);
@@ -689,20 +698,19 @@ static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D,
   const float c = fmaxf(fabsf(a.scale_log2), 0x1p-120f);
   if (steps > 0) { load(0); store(0); }
   for (int i = 0; i < steps; ++i) {
-    const int kb = k0 + CK * i;
+    const int kb = key_of(i);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();                             // stage i is whole, and the other one free
     asm volatile("" ::: "memory");
     if (i + 1 < steps) {
-      if (((kb + 2 * CK) >> 4) - first > F::PAGES) {          // the window of pages moves on (uniform, every 16 PAGES keys)
+      if (((key_of(i + 1) + CK) >> 4) - first > F::PAGES) {   // the window of pages moves on (uniform, every 16 PAGES keys, in their order)
         fill(kb >> 4);
-        __syncthreads();
       }
       load(i + 1);
     }
     if (!idle) {
     const unsigned char* ring = sm.ring[i & 1];
-    const bool paged = sm.page[(kb >> 4) - first + (CK == 64 ? g : g >> 1)] >= 0, plain = kb + CK <= base && !__any(!paged);
+    const bool plain = kb + CK <= base && !holes;
 #pragma unroll 1
     for (int e = 0; e < CK / 32; ++e) {                       // tiles 2 e, 2 e + 1: eight neighbouring keys of a lane group's
       f32x4 sc[RF][2];
@@ -727,6 +735,7 @@ static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D,
       __builtin_amdgcn_sched_barrier(0);
       bf16x8 pf[RF][1];
       if (!plain) {
+        const bool paged = sm.page[(kb >> 4) - first + (CK == 64 ? g : g >> 1)] >= 0;
 #pragma unroll
         for (int f = 0; f < RF; ++f) hide(sc[f], paged ? row_window<CK>(a, kb, base, h.ctx, row0 + 16 * f + rl, h.qlen, qstart, g) >> (8 * e) : 0u);
       }
@@ -765,8 +774,9 @@ static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D,
 
 template <int D, int RF> __global__ void __launch_bounds__(64 * NW, 2) tree_wide_kernel(TreeArgs a) {
   __shared__ WideSmem<D, RF> sm;
-  walk(a, Wide<D, RF>::R, [&](int seq, int qstart, const Shape& h, int kvh, int blk, int k0, int k1, int slot) __attribute__((always_inline)) {
-    wide_piece<D, RF>(a, sm, seq, qstart, h, kvh, blk, k0, k1, slot);
+  if (threadIdx.x == 0) sm.holes = 0;
+  walk(a, Wide<D, RF>::R, [&](int seq, int qstart, const Shape& h, int kvh, int blk, int k0, int k1, int turn, int slot) __attribute__((always_inline)) {
+    wide_piece<D, RF>(a, sm, seq, qstart, h, kvh, blk, k0, k1, turn, slot);
   });
 }
 

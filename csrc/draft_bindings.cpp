@@ -142,7 +142,7 @@ Tensor tree_attention(Tensor q, Tensor k, Tensor v, Tensor bt, Tensor qstart, Te
   int64_t ulen = keys <= 256 ? 0 : wide ? 64 : c.eight && rf == 1 ? 256 : 128;
   const int64_t way = wide ? 4 : rf > 1 ? 3 : c.eight ? 1 : 0, least = ulen ? (keys > 4096 ? 512 : 256) / ulen : 1;
   // the list of units is counted in 32 bits
-  NEED(c.nkv < 65536, "tree_attention: too many heads");
+  NEED(c.nkv < (1 << 20), "tree_attention: too many heads");
   const int64_t listed = c.nkv * (T * G / R + S);
   NEED(T * nq <= 0x7fffffff && listed < (1 << 30), "tree_attention: too many");
   while (ulen && listed * (max_blocks * BS / ulen + 1 + way) >= (1 << 30)) ulen *= 2;

@@ -662,7 +662,7 @@ static __device__ __forceinline__ void wide_piece(const TreeArgs& a, WideSmem<D,
                         : (16 * (own % NT) + rl) * BS + (CK == 64 ? 8 * (own / NT) : 8 * (g & 1));
   const u16* lane_src = (const u16*)(of_k ? a.kc : a.vc) + (long)kvh * BS * D + from;
   const int lane_page = CK == 64 ? (of_k ? rl >> 2 : g) : (of_k ? rl >> 3 : g >> 1);
-  const uint32_t page_len = (uint32_t)a.nkv * BS * D;         // (the launcher: fewer than 2^16 kv heads)
+  const uint32_t page_len = (uint32_t)a.nkv * BS * D;         // (fewer than 2^20 kv heads: fits)
   int page = 0;
   auto load = [&](int i) {
     page = sm.page[(key_of(i) >> 4) - first + lane_page];

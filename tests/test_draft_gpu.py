@@ -256,6 +256,23 @@ def test_pages_outside_the_pool_are_not_seen(eight):
     near(attend(to(s, DEV)), want, bound)
 
 
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_row_blocks_cut_at_different_keys(eight, d):
+    """Several row blocks over the same keys, each in parts of its own: parts begin in their middle.  Pages outside the pool anywhere on the way, the last
+    one of a sequence too."""
+    s = step([(75, 3001), (41, 1500), (20, 777)], 8, 2, d, eight, "tree", 19)
+    see = [visible(s, b) for b in range(3)]
+    for b, page in ((0, 0), (0, 31), (0, 100), (0, 187), (1, 64), (1, 93), (2, 48)):
+        see[b][:, page * BS:(page + 1) * BS] = False
+    want, bound = attention64(s, see)
+    whole = attention64(s)
+    near(attend(to(s, DEV)), *whole)
+    for b, page in ((0, 0), (0, 31), (0, 100), (0, 187), (1, 64), (1, 93), (2, 48)):
+        s["table"][b, page] = -1 if page % 2 else s["k"].shape[0]
+    near(attend(to(s, DEV)), want, bound)
+
+
 def test_a_row_that_sees_nothing_is_zero():
     s = step([(6, 6), (3, 40)], 8, 2, 64, False, "tree", 4)
     s["mask"][2] = 0

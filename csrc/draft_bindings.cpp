@@ -125,7 +125,7 @@ Tensor tree_attention(Tensor q, Tensor k, Tensor v, Tensor bt, Tensor qstart, Te
   const int64_t keys = std::min(max_ctx ? max_ctx : max_blocks * BS, max_blocks * BS);
   // Rows of a wave, and whether four waves have rows of their own over shared keys (bf16).  us, sequences of 200 to 3000 keys, 8 kv heads of 128, one
   // wave's 16 / 32 / 48 rows, four waves' 64 / 128: 48 rows 65 / 61 / 58, 54 / 63; 80 to 160 rows 163 / 117 / 115, 104 / 82; 512 rows of 8000 to 32000
-  // keys 940 / 389 / 327, 281 / 203.  e4m3 keys cost conversions in every wave that shares them, or LDS bandwidth as bf16: the last one 488 / 217 / 182
+  // keys 940 / 389 / 327, 281 / 203 (four waves' after that, with one address a chunk and finer units: 48 rows 42, then 65 and 178).  e4m3 keys cost conversions in every wave that shares them, or LDS bandwidth as bf16: the last one 488 / 217 / 182
   // and 286 / 211, 48 rows 46 / 41 / 37 and 43 / 51.
   // What fits the chip at once in 16-row blocks is cut that fine, for the shortest way through (one chat of 437 keys, 40 rows: 12.2 us, 10.4 so).
   const int64_t fine = S * c.nkv * ((most + 15) / 16) * ((keys + 255) / 256);

@@ -10,15 +10,16 @@
 //
 // Few rows (up to 32; e4m3: any number, 48 at a time): a workgroup is four waves over the same 16 RF rows (heads of one kv head, tokens x group), each
 // with its own chunks.  K and V go to registers once for all rows and are never staged; the waves meet in LDS at the end.  Bound by memory: 64
-// single tokens of 500 to 6000 keys, 8 kv heads of 128, 114 us (5.1 TB/s), over e4m3 68 (4.4).  More rows: tree_wide_kernel below.
+// single tokens of 500 to 6000 keys, 8 kv heads of 128, 112 us (5.2 TB/s), over e4m3 66 (4.5).  More rows: tree_wide_kernel below.
 //
 // e4m3 caches: codes become bf16 exactly (three bits behind the leading one), the key's scale multiplies its score and the value's its weight,
 // ahead of the weight's rounding to bf16; the sum of weights is of the unrounded ones.
 //
 // Split: all (sequence, kv head, row block, range of `ulen` keys) form one list, cut into equal parts for the workgroups that fit the chip at
-// once; a row block counts for some units more than its keys, for the way in and out of it (queries, masks, sums).  Every workgroup finds its part from the lengths on the device, so ragged batches are even, nothing is planned on the host and a
-// captured graph takes new lengths.  A part's first and last piece may be of a row block that others hold too: their sums go to the workspace
-// in 32 bits and a second launch joins them, in order (no atomics: the same bits every time).
+// once; a row block counts for some units more than its keys, for the way in and out of it (queries, masks, sums).  Every workgroup finds its
+// part from the lengths on the device, so ragged batches are even, nothing is planned on the host and a captured graph takes new lengths.  A
+// part's first and last piece may be of a row block that others hold too: their sums go to the workspace in 32 bits and a second launch joins
+// them, in order (no atomics: the same bits every time).
 #include "common.h"
 
 namespace {
@@ -527,7 +528,8 @@ static __device__ __forceinline__ void piece(const TreeArgs& a, TreeSmem<D, RF, 
 
 // A workgroup's part of the list: run(sequence, its first row, its shape, kv head, row block, first key, last key, turn, slot) for every piece of it.
 // A piece begins `turn` keys behind its first one and comes to those in the end: parts of the row blocks of a kv head, which read the same keys and are cut at
-// different ones, are so at the same keys (modulo a part) at the same time, and find them in L2.
+// different ones, are so at the same keys (modulo a part) at the same time, and find them in L2 (512 rows of 8000 to 32000 keys: 8.3 M misses, 4.4 M so;
+// 5 us of 195).
 template <class F> static __device__ __forceinline__ void walk(const TreeArgs& a, int R, F&& run) {
   const List q = scan_units(a, R);
   const bool lead = threadIdx.x == 0 && a.joins;
@@ -587,9 +589,9 @@ __global__ void __launch_bounds__(64 * NW, (RF > 1 || D > 64 ? 2 : 3)) tree_attn
 // Four waves of 16 RF rows read every chunk from LDS, in two stages: a wave asks for its share of the next chunk, computes on this one and then writes
 // what has arrived.  One operand fragment is a kilobyte in lane order, read back as it lies, without conflicts.  K and V leave L2 once for 64 RF
 // rows: with rows of one wave only, every 48 read them again, and ragged trees of 80 to 160 rows (8 kv heads of 128, 32 sequences of 200 to 3000 keys)
-// ran at what L2 misses of four such readings allow (115 us, 82 so).  512 rows of 8000 to 32000 keys: 203 us, 555 TFLOP/s; two waves a SIMD that wait for
-// the same chunk leave a quarter of the matrix cores' time used, and L2 misses of the row blocks take 5.2 TB/s.  (Loads straight to LDS made the compiler wait for all of
-// them ahead of any LDS read; 48 rows a wave spill, 64 keys a stage gain nothing.)
+// ran at what L2 misses of four such readings allow (115 us, 65 so).  512 rows of 8000 to 32000 keys: 178 us, 630 TFLOP/s; vector instructions take 42 %
+// of the time and products 38, and two waves a SIMD hardly overlap them.  (Loads straight to LDS made the compiler wait for all of them ahead of
+// any LDS read; 48 rows a wave spill; 64 keys a stage, loads two chunks ahead and a higher priority within products gain nothing.)
 template <int D, int RF> struct Wide {
   static constexpr int CK = D > 64 ? 32 : 64, KS = D / 32, NT = D / 16, TL = CK / 16, KPG = CK / 4, R = 16 * RF * NW;
   // one-kilobyte slots of a stage: K a tile and 32 dims (slot t * KS + s), V eight keys a lane group and sixteen dims (KSL + e * NT + n)

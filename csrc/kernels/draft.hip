@@ -11,17 +11,22 @@ constexpr int NTH = 256;
 
 // ------------------------------------------------------------------------------------------------ masks
 // Workgroup s < S: a node's word of ancestors (itself among them) and their number, from a walk up the parents in LDS; indices fall on the way,
-// so a word is whole when the walk leaves it (32 trees of 20 to 40 nodes 4 us, a launch's own time).  Workgroups behind: rows that no sequence has, or that lie past 32 W nodes of it, become zero.
+// so a word is whole when the walk leaves it (32 trees of 20 to 40 nodes 4 us, a launch's own time).  Workgroups behind: rows that no sequence has, or that lie past 32 W nodes of it, become
+// zero; a thread looks at every 256th sequence and marks what it has of the workgroup's rows (a row that looks for its sequence by itself: 512 sequences 70 us, 4 so).
 __global__ void __launch_bounds__(NTH) tree_mask_kernel(const int* __restrict__ parents, const int* __restrict__ qstart, const int* __restrict__ qlen,
                                                         int* __restrict__ mask, int* __restrict__ depth, int W, int S, int T) {
   __shared__ int par[MAX_NODES];
   if ((int)blockIdx.x >= S) {
-    const int t = (blockIdx.x - S) * NTH + threadIdx.x;
-    if (t >= T) return;
-    for (int s = 0; s < S; ++s) {
+    const int t0 = (blockIdx.x - S) * NTH, t = t0 + threadIdx.x;
+    par[threadIdx.x] = 0;
+    __syncthreads();
+    for (int s = threadIdx.x; s < S; s += NTH) {
       const int q0 = qstart[s], n = min(qlen[s], 32 * W);
-      if (t >= q0 && t - q0 < n && q0 >= 0 && q0 <= T - n) return;
+      if (n <= 0 || q0 < 0 || q0 > T - n) continue;
+      for (int i = max(q0, t0); i < min(q0 + n, t0 + NTH); ++i) par[i - t0] = 1;
     }
+    __syncthreads();
+    if (t >= T || par[threadIdx.x]) return;
     for (int w = 0; w < W; ++w) mask[(long)t * W + w] = 0;
     depth[t] = 0;
     return;

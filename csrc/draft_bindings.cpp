@@ -136,11 +136,12 @@ Tensor tree_attention(Tensor q, Tensor k, Tensor v, Tensor bt, Tensor qstart, Te
   const int64_t blocks = S * c.nkv * ((most + R - 1) / R);      // row blocks, at most
   // Keys of a unit (of whole rounds of a workgroup's chunks), units that a row block's way in and out counts for, and units of a part, at least: short
   // parts of long contexts leave many pieces to join.  us with a way of 0 / 2 / 3 / 4 / 6 units: ragged trees of 80 to 160 rows 94 / 78 / 75 / 74 / 75, 160
-  // rows of a chain 108 / 91 / 87 / 86 / 92; 48 rows over e4m3 39 / 37 / 35 / 35 / 36; 16 rows are bound by memory, 64 single tokens 113 / 116 / 118.
+  // rows of a chain 108 / 91 / 87 / 86 / 92; 48 rows over e4m3 39 / 37 / 35 / 35 / 36; 16 rows are bound by memory, 64 single tokens of up to 6000 keys
+  // 113 / 116 / 118 (0 / 1 / 2 units where contexts are shorter: 512 of 200 to 1000 keys, 4 kv heads of 64, 68 / 65 / 65; 2000 of 100 to 400 146 / 141 / 140).
   // With units of 256 keys and no way 82, 100, 37, 113.  Parts of 512 keys and more from 4096 on: one sequence of 16000 65 -> 55.  A context of up to
   // 256 keys is one unit, not split: one launch.
   int64_t ulen = keys <= 256 ? 0 : wide ? 64 : c.eight && rf == 1 ? 256 : 128;
-  const int64_t way = wide ? 4 : rf > 1 ? 3 : c.eight ? 1 : 0, least = ulen ? (keys > 4096 ? 512 : 256) / ulen : 1;
+  const int64_t way = wide ? 4 : rf > 1 ? 3 : c.eight || keys <= 4096 ? 1 : 0, least = ulen ? (keys > 4096 ? 512 : 256) / ulen : 1;
   // the list of units is counted in 32 bits
   NEED(c.nkv < (1 << 20), "tree_attention: too many heads");
   const int64_t listed = c.nkv * (T * G / R + S);

@@ -89,7 +89,7 @@ def verify(target: torch.Tensor, tokens: torch.Tensor, uniform: torch.Tensor, se
       no ``draft``: given candidates, a tree by ``parents`` or a chain.  A node's children are tried in order, each against what the earlier ones left
       of the target: u (1 - what they held) < target; the last draw leaves the refused children's tokens out.
     ``path``: the root and the accepted nodes, -1 behind them.  A sequence without nodes gets 0 accepted and token -1.  Sums and products are of 64
-    bits: the same tokens as any other order would give."""
+    bits."""
     ext = _native(target)
     if ext is not None:
         return ext.verify_drafts(target, tokens, uniform, seq_qstart, seq_qlen, max_nodes, parents, draft)

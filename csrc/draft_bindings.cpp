@@ -139,8 +139,9 @@ Tensor tree_attention(Tensor q, Tensor k, Tensor v, Tensor bt, Tensor qstart, Te
   // rows of a chain 108 / 91 / 87 / 86 / 92; 48 rows over e4m3 39 / 37 / 35 / 35 / 36; 16 rows are bound by memory, 64 single tokens of up to 6000 keys
   // 113 / 116 / 118 (0 / 1 / 2 units where contexts are shorter: 512 of 200 to 1000 keys, 4 kv heads of 64, 68 / 65 / 65; 2000 of 100 to 400 146 / 141 / 140).
   // With units of 256 keys and no way 82, 100, 37, 113.  Parts of 512 keys and more from 4096 on: one sequence of 16000 65 -> 55.  A context of up to
-  // 256 keys is one unit, not split: one launch.
-  int64_t ulen = keys <= 256 ? 0 : wide ? 64 : c.eight && rf == 1 ? 256 : 128;
+  // 512 keys is one unit, not split: one launch (us in a graph with a bound of 256 / 512 / 1024 keys: one chat of 437, masks beside it, 10.7 / 9.0 / 9.0; 64 of
+  // 300 to 500 20 / 16.5 / 16.4; one of 800 and 40 nodes 22 / 22 / 33; 512 of up to 1000 and 5 nodes 86 / 86 / 101).
+  int64_t ulen = keys <= 512 ? 0 : wide ? 64 : c.eight && rf == 1 ? 256 : 128;
   const int64_t way = wide ? 4 : rf > 1 ? 3 : c.eight || keys <= 4096 ? 1 : 0, least = ulen ? (keys > 4096 ? 512 : 256) / ulen : 1;
   // the list of units is counted in 32 bits
   NEED(c.nkv < (1 << 20), "tree_attention: too many heads");

@@ -127,7 +127,7 @@ Tensor tree_attention(Tensor q, Tensor k, Tensor v, Tensor bt, Tensor qstart, Te
   // wave's 16 / 32 / 48 rows, four waves' 64 / 128: 48 rows 65 / 61 / 58, 54 / 63; 80 to 160 rows 163 / 117 / 115, 104 / 82; 512 rows of 8000 to 32000
   // keys 940 / 389 / 327, 281 / 203 (four waves' after that, with one address a chunk and finer units: 48 rows 42, then 65 and 178).  e4m3 keys cost conversions in every wave that shares them, or LDS bandwidth as bf16: the last one 488 / 217 / 182
   // and 286 / 211, 48 rows 46 / 41 / 37 and 43 / 51.
-  // What fits the chip at once in 16-row blocks is cut that fine, for the shortest way through (one chat of 437 keys, 40 rows: 12.2 us, 10.4 so).
+  // What fits the chip at once in 16-row blocks is cut that fine, for the shortest way through (one chat of 437 keys, 40 rows, in two launches: 12.2 us, 10.4 so).
   const int64_t fine = S * c.nkv * ((most + 15) / 16) * ((keys + 255) / 256);
   const bool wide = !c.eight && most > 32 && fine > cus(q);
   const int rf = wide ? (most <= 64 ? 1 : 2) : most <= 16 || fine <= cus(q) ? 1 : most <= 32 ? 2 : 3;

@@ -258,6 +258,17 @@ def test_pages_outside_the_pool_are_not_seen(eight):
 
 @pytest.mark.parametrize("eight", [False, True])
 @pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("most", [512, 513])
+def test_the_longest_contexts_of_one_launch(eight, d, most):
+    """Tables of 32 blocks are not cut, of 33 they are: rows of every form."""
+    s = step([(64, most), (33, 511), (1, 500), (16, 480), (0, 70), (5, 5)], 8, 2, d, eight, "tree", 21)
+    want, bound = attention64(s)
+    near(attend(to(s, DEV)), want, bound)
+    near(attend(to(s, DEV), max_qlen=64, max_ctx=most), want, bound)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("d", [64, 96, 128])
 def test_row_blocks_cut_at_different_keys(eight, d):
     """Several row blocks over the same keys, each in parts of its own: parts begin in their middle.  Pages outside the pool anywhere on the way, the last
     one of a sequence too."""
@@ -486,6 +497,24 @@ def test_masks(lens, most):
     par[sum(lens) - 1] = 10 ** 6                                # a parent behind its child counts as none
     start, n = i32([sum(lens[:i]) for i in range(len(lens))]), i32(lens)
     want, got = ref.tree_mask(par, start, n, most), ops.draft.tree_mask(par.to(DEV), start.to(DEV), n.to(DEV), most)
+    assert torch.equal(want[0], got[0].cpu()) and torch.equal(want[1], got[1].cpu())
+
+
+def test_masks_of_many_sequences_with_rows_between():
+    """700 sequences in rows of their own order, rows of none between them: more than one workgroup has of either."""
+    rng = random.Random(9)
+    lens = [rng.choice([0, 1, 2, 5, 9]) for _ in range(700)]
+    starts, at = [], 0
+    for n in lens:
+        at += rng.choice([0, 0, 1, 3])
+        starts.append(at)
+        at += n
+    par = [5] * (at + 300)
+    for q0, n in zip(starts, lens):
+        par[q0:q0 + n] = tree(rng, n)
+    order = rng.sample(range(700), 700)
+    start, n = i32([starts[i] for i in order]), i32([lens[i] for i in order])
+    want, got = ref.tree_mask(i32(par), start, n, 9), ops.draft.tree_mask(i32(par, DEV), start.to(DEV), n.to(DEV), 9)
     assert torch.equal(want[0], got[0].cpu()) and torch.equal(want[1], got[1].cpu())
 
 

@@ -161,6 +161,9 @@ template <class T> static __device__ __forceinline__ bool vectors(const VerifyAr
   return !((uintptr_t)a.target & m) && !(a.target_ld * sizeof(T) & m) && !((uintptr_t)a.draft & m) && (!a.draft || !(a.draft_ld * sizeof(T) & m));
 }
 
+// What earlier siblings left of the target, 0 at least; a NaN among them stays one (fmax would make it 0, and any later sibling would be accepted).
+static __device__ __forceinline__ double left(double mass) { return mass < 0.0 ? 0.0 : mass; }
+
 // Where the accepted path ends, and its length, of more than 64 nodes: a thread a node, in LDS.
 template <class T> static __device__ __forceinline__ void tree_walk(const VerifyArgs& a, VerifySmem& sm, int q0, int n, int& last, int& len) {
   const T *target = (const T*)a.target, *draft = (const T*)a.draft;
@@ -196,7 +199,7 @@ template <class T> static __device__ __forceinline__ void tree_walk(const Verify
         double mass = 1.0;
         for (int j = sm.par[i] + 1; j < i; ++j)
           if (sm.par[j] == sm.par[i]) mass -= sm.px[j];
-        sm.ok[i] = sm.tok[i] >= 0 && sm.tok[i] < a.V && (double)a.uniform[q0 + i] * fmax(mass, 0.0) < sm.px[i];
+        sm.ok[i] = sm.tok[i] >= 0 && sm.tok[i] < a.V && (double)a.uniform[q0 + i] * left(mass) < sm.px[i];
       }
     __syncthreads();
   }
@@ -248,7 +251,7 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_walk_kernel(Ver
           if (x == xj) px = 0.0;
         }
       }
-    bool take = real && (draft ? u * (double)val<T>(draft + (long)(q0 + i) * a.draft_ld + x) < px : u * fmax(mass, 0.0) < px);
+    bool take = real && (draft ? u * (double)val<T>(draft + (long)(q0 + i) * a.draft_ld + x) < px : u * left(mass) < px);
     for (unsigned long long m = __ballot(take); m; m &= m - 1) {     // a parent's first accepted child
       const int j = __builtin_ctzll(m), pj = __builtin_amdgcn_readlane(par, j);
       if (i > j && par == pj) take = false;

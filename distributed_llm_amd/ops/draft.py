@@ -88,6 +88,7 @@ def verify(target: torch.Tensor, tokens: torch.Tensor, uniform: torch.Tensor, se
       u draft < target, and the last draw is from max(target - draft, 0) of the refused node, or from the target behind the last one.
       no ``draft``: given candidates, a tree by ``parents`` or a chain.  A node's children are tried in order, each against what the earlier ones left
       of the target: u (1 - what they held) < target; the last draw leaves the refused children's tokens out.
+    A NaN accepts nothing, nor do candidates behind it, of whose parent it leaves no number; the last draw takes it for 0.
     ``path``: the root and the accepted nodes, -1 behind them.  A sequence without nodes gets 0 accepted and token -1.  Sums and products are of 64
     bits."""
     ext = _native(target)

@@ -1,0 +1,44 @@
+"""Drafted tokens at the edges of what their calls allow: kernels against their definitions and against the CPU forms."""
+import math
+
+import pytest
+import torch
+
+from distributed_llm_amd import ops
+from draft_cases import i32
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _native():
+    assert ops.native_available(), "HIP extension must be built for GPU tests"
+
+
+# ------------------------------------------------------------------------------------------------ verification
+def verified(s, most):
+    """The same from both forms of the call; what they say."""
+    args = [s[t] for t in ("target", "tokens", "uniform", "qstart", "qlen")]
+    kw = {t: s.get(t) for t in ("parents", "draft")}
+    want = ops.draft.verify(*args, most, **kw)
+    got = ops.draft.verify(*[x.to(DEV) for x in args], most, **{t: None if x is None else x.to(DEV) for t, x in kw.items()})
+    for a, b in zip(want, got):
+        assert torch.equal(a, b.cpu())
+    return [x.tolist() for x in want]
+
+
+@pytest.mark.parametrize("nodes", [3, 64, 65, 90])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_candidates_behind_a_nan_are_refused(nodes, dtype):
+    """What a NaN leaves of the target is no number, so nothing compares below a later sibling's probability; the earlier ones are tried as ever.  Lanes
+    hold trees of up to 64 nodes, LDS larger ones; the nodes behind the third hang on it."""
+    V = 40
+    for at, want in ((1, 0), (2, 1)):                           # the NaN ahead of the likely candidate, and behind it
+        target = torch.full((nodes, V), 1.0 / V).to(dtype)
+        target[0, 7], target[0, 9] = (math.nan, 0.25) if at == 1 else (0.95, math.nan)
+        s = dict(target=target, tokens=i32([0, 7, 9] + [3] * (nodes - 3)), uniform=torch.full((nodes,), 0.9), qstart=i32([0]), qlen=i32([nodes]),
+                 parents=i32([-1, 0, 0] + list(range(2, nodes - 1))))
+        accepted, token, _ = verified(s, nodes)
+        assert accepted == [want]
+        assert want or token[0] not in (7, 9)

@@ -360,9 +360,10 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_pick_kernel(Ver
     __syncthreads();
     return x;
   };
-  // The first thread whose sum passes t, NTH if none does (not the one between two sums: rounding may leave sums of neighbours in the wrong order).
-  auto first_over = [&](double sum, double t) {
-    const unsigned long long over = __ballot(sum > t);
+  // The first thread with weight whose sum passes t, NTH if none does (not the one between two sums: rounding may leave sums of neighbours in the wrong
+  // order, and a thread without weight a bit above the one before it).
+  auto first_over = [&](double own, double sum, double t) {
+    const unsigned long long over = __ballot(own > 0.0 && sum > t);
     if (lane == 0) sm.wlast[wid][1] = over ? 64 * wid + __builtin_ctzll(over) : NTH;
     __syncthreads();
     int m = NTH;
@@ -384,7 +385,7 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_pick_kernel(Ver
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) l = max(l, __shfl_xor(l, o, 64));
   if (lane == 0) sm.wlast[wid][0] = l;
-  const int part = first_over(incl, t);
+  const int part = first_over(which ? own_p : mine, incl, t);
   if (part >= a.P) {                                                 // (infinite sums, or u = 1)
     if (tid == 0) {
       int m = -1;
@@ -416,23 +417,23 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_pick_kernel(Ver
     own += x[0]; own += x[1]; own += x[2]; own += x[3];
   }
   const double up = base + scan(own), down = tid ? base + cum[tid - 1] : base;
-  const int who = first_over(up, t);
+  const int who = first_over(own, up, t);
   if (who == NTH && tid == 0) a.next[s] = max(lasts[2 * part + which], 0);
   if (tid == who) {
     double run = down;
     int got = -1;
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      if (w[j] > 0.0 && !(run > t)) { run += w[j]; got = from + j; }
+      if (w[j] > 0.0 && (got < 0 || !(run > t))) { run += w[j]; got = from + j; }
     for (int v = from + 16; v < to; v += 4) {
       double x[4];
       fetch(p, q, v, to, vec, f4[0], h4[0]);
       weights(f4[0], h4[0], v, sm, x, pw);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (x[j] > 0.0 && !(run > t)) { run += x[j]; got = v + j; }
+        if (x[j] > 0.0 && (got < 0 || !(run > t))) { run += x[j]; got = v + j; }
     }
-    a.next[s] = got >= 0 ? got : max(lasts[2 * part + which], 0);
+    a.next[s] = got;
   }
 }
 

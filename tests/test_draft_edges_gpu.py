@@ -42,3 +42,14 @@ def test_candidates_behind_a_nan_are_refused(nodes, dtype):
         accepted, token, _ = verified(s, nodes)
         assert accepted == [want]
         assert want or token[0] not in (7, 9)
+
+
+def test_a_part_without_weight_is_not_drawn_from():
+    """Running sums of parts of 4096 tokens meet in an order of their own: here the sum up to the fifth part, which has no weight, rounds to one bit more
+    than the one up to the fourth, and u times the whole lies between them.  The draw is one of the tokens with weight, the same from both forms."""
+    V, e = 6 * 4096, 2.0 ** -54
+    target = torch.zeros(1, V)
+    for at, p in ((7, 0.5), (4096 + 5, e), (3 * 4096 + 6, e), (5 * 4096 + 8, 0.5)):
+        target[0, at] = p
+    _, token, _ = verified(dict(target=target, tokens=i32([0]), uniform=torch.tensor([0.5]), qstart=i32([0]), qlen=i32([1])), 1)
+    assert token == [5 * 4096 + 8]

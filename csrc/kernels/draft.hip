@@ -235,7 +235,7 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_walk_kernel(Ver
   int* path = a.path + (long)s * a.N;
   int last = 0, len = 1;
   bool refused;
-  const int v0 = blockIdx.x * a.part, v1 = min(a.V, v0 + a.part);
+  const int v0 = blockIdx.x * a.part, v1 = v0 + min(a.V - v0, a.part);      // (a whole last part may end past 2^31)
   if (n <= 64) {
     // a lane a node, in every wave by itself, without LDS (trees of 40 nodes: 16 us of a launch in LDS, 11 so)
     const int i = tid & 63, x = i < n ? a.tokens[q0 + i] : -1, par = i < n ? parent_of(a, q0, i) : -3;
@@ -395,12 +395,12 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_pick_kernel(Ver
     return;
   }
   const double base = part ? cum[part - 1] : 0.0;
-  const int v0 = part * a.part, v1 = min(a.V, v0 + a.part), each = a.part / NTH;
+  const int v0 = part * a.part, v1 = v0 + min(a.V - v0, a.part), each = a.part / NTH;
   left_out(a, sm, which ? 0 : n, last, v0, v1);
   const T* p = (const T*)a.target + (long)(q0 + last) * a.target_ld;
   const T* q = a.draft && f[1] && !which ? (const T*)a.draft + (long)(q0 + last + 1) * a.draft_ld : nullptr;
   const bool vec = vectors<T>(a);
-  const int from = v0 + tid * each, to = min(v1, from + each);
+  const int from = v0 + tid * each, to = from + min(v1 - from, each);
   // sixteen weights of a thread stay in registers; longer rows than 16 NTH NTH read theirs again
   double w[16], pw[4], own = 0.0;
   float f4[4][4], h4[4][4];
@@ -529,9 +529,9 @@ extern "C" int dllm_tree_mask(const int* parents, const int* qstart, const int* 
 // Parts of a row: `part` values each, at most NTH of them.
 extern "C" int dllm_verify_parts(int V, int* part) {
   int p = 16 * NTH;
-  while ((V + p - 1) / p > NTH) p *= 2;
+  while (((long)V + p - 1) / p > NTH) p *= 2;
   *part = p;
-  return (V + p - 1) / p;
+  return (int)(((long)V + p - 1) / p);
 }
 
 extern "C" int dllm_verify(const void* target, long target_ld, const void* draft, long draft_ld, int bf16, const int* tokens, const int* parents,

@@ -53,3 +53,12 @@ def test_a_part_without_weight_is_not_drawn_from():
         target[0, at] = p
     _, token, _ = verified(dict(target=target, tokens=i32([0]), uniform=torch.tensor([0.5]), qstart=i32([0]), qlen=i32([1])), 1)
     assert token == [5 * 4096 + 8]
+
+
+def test_the_last_tokens_of_the_largest_vocabulary():
+    """0x7fff0000 tokens, the most that a call takes: the last part ends past 2^31 if it is whole."""
+    V = 0x7FFF0000
+    target = torch.zeros(1, V, dtype=torch.bfloat16, device=DEV)
+    target[0, V - 1] = 0.75
+    got = ops.draft.verify(target, i32([0], DEV), torch.tensor([0.5], device=DEV), i32([0], DEV), i32([1], DEV), 1)
+    assert [t.tolist() for t in got] == [[0], [V - 1], [[0]]]

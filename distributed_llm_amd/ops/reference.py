@@ -1209,7 +1209,7 @@ def tree_attention(q, k_cache, v_cache, block_tables, seq_qstart, seq_qlen, seq_
     out = torch.zeros_like(q)
     for s in range(block_tables.shape[0]):
         q0, n = int(seq_qstart[s]), int(seq_qlen[s])
-        ctx = min(int(seq_ctx[s]), block_tables.shape[1] * BS)
+        ctx = min(int(seq_ctx[s]), block_tables.shape[1] * BS if nb else 0)
         rows = [i for i in range(n) if 0 <= q0 + i < T]
         if not rows or ctx <= 0:
             continue

@@ -98,7 +98,7 @@ Tensor tree_attention(Tensor q, Tensor k, Tensor v, Tensor bt, Tensor qstart, Te
   NEED(c.nkv >= 1 && nq >= 1 && nq % c.nkv == 0, "query heads must be a multiple of the cache's");
   same_device(q, bt, "block_tables");
   NEED(bt.dim() == 2 && bt.scalar_type() == at::kInt && bt.is_contiguous(), "block_tables: contiguous int32 [num_seqs, max_blocks]");
-  const int64_t S = bt.size(0), max_blocks = bt.size(1);
+  const int64_t S = bt.size(0), max_blocks = c.blocks ? bt.size(1) : 0;      // (an empty pool has no key for any table)
   vec_i32(q, qstart, "seq_qstart", S);
   vec_i32(q, qlen, "seq_qlen", S);
   vec_i32(q, ctx, "seq_ctx", S);
@@ -119,7 +119,7 @@ Tensor tree_attention(Tensor q, Tensor k, Tensor v, Tensor bt, Tensor qstart, Te
   for (int64_t n : {T, nq, S, max_blocks * BS, c.blocks}) check_int(n, "tree_attention");
   const c10::OptionalDeviceGuard guard(q.device());
   Tensor o = out ? *out : at::empty({T, nq, d}, q.options());
-  if (T == 0 || S == 0 || max_blocks == 0 || c.blocks == 0) return o;
+  if (T == 0 || S == 0) return o;
   const int64_t G = nq / c.nkv;
   const int64_t most = std::min(max_qlen ? max_qlen : S == 1 ? T : W ? 32 * W : T, T) * G;
   const int64_t keys = std::min(max_ctx ? max_ctx : max_blocks * BS, max_blocks * BS);

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from distributed_llm_amd import ops
-from draft_cases import i32
+from draft_cases import attend, i32, step, to
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -62,3 +62,25 @@ def test_the_last_tokens_of_the_largest_vocabulary():
     target[0, V - 1] = 0.75
     got = ops.draft.verify(target, i32([0], DEV), torch.tensor([0.5], device=DEV), i32([0], DEV), i32([1], DEV), 1)
     assert [t.tolist() for t in got] == [[0], [V - 1], [[0]]]
+
+
+# ------------------------------------------------------------------------------------------------ attention
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("what", ["no column in the tables", "no block in the pool"])
+def test_no_key_at_all_gives_rows_of_zeros(eight, d, what):
+    """Rows of the sequences become zero, rows behind the last one stay what they were, as in the CPU form."""
+    s = step([(5, 40), (1, 3), (0, 0), (70, 90)], 8, 2, d, eight, "tree", 5, pad=3)
+    if what.startswith("no column"):
+        s["table"] = s["table"][:, :0].contiguous()
+    else:
+        for t in ("k", "v", "ks", "vs"):
+            s[t] = None if s[t] is None else s[t][:0]
+    for mask in (s["mask"], None):
+        outs = []
+        for h in (dict(s, mask=mask), to(dict(s, mask=mask), DEV)):
+            out = torch.full((79, 8, d), 7.0, dtype=torch.bfloat16, device=h["q"].device)
+            attend(h, out=out)
+            assert not attend(h)[:76].any()
+            outs.append(out.cpu())
+        assert torch.equal(*outs) and not outs[1][:76].any() and bool((outs[1][76:] == 7.0).all())

@@ -846,7 +846,8 @@ template <int D> int launch_d(const TreeArgs& a, int rf, bool wide, int rows, hi
 }
 }  // namespace
 
-// rf: a wave has 16 rf rows (bf16 1 or 2, e4m3 up to 3).  wide (bf16): a row block is four waves' rows, else one's.  ulen: keys of a unit, a multiple of 64; 0: a row block is
+// rf: a wave has 16 rf rows (bf16 1 or 2, e4m3 up to 3).  wide (bf16): a row block is four waves' rows, else one's.  ulen: keys of a unit, whole rounds of a workgroup's
+// chunks (64 keys wide, 256 of e4m3 in 16 rows, else 128), since a piece begins units behind its first key and goes on in rounds; 0: a row block is
 // one unit (no workspace, one launch).  max_blocks of 0: no sequence has a key, nothing is read but the lengths and queries, and all rows are zero.  way: units that a row block counts for beside its keys; least: units of a part.  rows: those of a block that the join's grid has waves for.
 extern "C" int dllm_tree_attention(const void* q, long q_ts, long q_hs, const void* kc, const void* vc, const float* ks, const float* vs,
                                    const int* bt, const int* qstart, const int* qlen, const int* ctx, const int* mask, void* out, float* part_o,
@@ -854,7 +855,8 @@ extern "C" int dllm_tree_attention(const void* q, long q_ts, long q_hs, const vo
                                    int rf, int wide, int rows, float scale, hipStream_t st) {
   if (nkv < 1 || nq < nkv || nq % nkv || rf < 1 || rf > 3 || rows < 1) return -1;
   if ((ks == nullptr) != (vs == nullptr) || S < 1 || T < 1 || max_blocks < 0 || num_blocks < 0 || (max_blocks && !num_blocks) || nwg < 1) return -2;
-  if (ulen < 0 || ulen % 64 || way < 0 || least < 1 || (ulen && (!part_o || !part_ml || !joins))) return -3;
+  const int round = wide ? 64 : ks && rf == 1 ? 256 : 128;
+  if (ulen < 0 || ulen % round || way < 0 || least < 1 || (ulen && (!part_o || !part_ml || !joins))) return -3;
   TreeArgs a{(const u16*)q, q_ts, q_hs, kc, vc, ks, vs, bt, qstart, qlen, ctx, mask, (u16*)out, part_o, part_ml,
              ulen ? joins : nullptr, W, S, T, nq, nkv, nq / nkv, max_blocks, num_blocks, nwg, ulen, ulen ? way : 0, ulen ? least : 1, scale * LOG2E};
   switch (d) {

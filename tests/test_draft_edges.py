@@ -1,7 +1,11 @@
 """Drafted tokens and the 8-bit cache at the edges of what their calls allow: the CPU forms, and refusals that need no GPU."""
+import ctypes
+
 import pytest
 import torch
 
+from distributed_llm_amd import ops
+from distributed_llm_amd._build import HIP_SO
 from draft_cases import attend, step
 
 
@@ -17,3 +21,21 @@ def test_no_key_at_all_gives_rows_of_zeros(eight, what):
     out = torch.full((9, 8, 64), 7.0, dtype=torch.bfloat16)
     attend(s, out=out)
     assert not out[:6].any() and bool((out[6:] == 7.0).all())
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="hands the launcher no real memory")
+@pytest.mark.parametrize("eight,rf,wide,units", [(False, 1, 0, 128), (False, 2, 0, 128), (True, 1, 0, 256), (True, 2, 0, 128), (True, 3, 0, 128),
+                                                 (False, 1, 1, 64), (False, 2, 1, 64)])
+def test_the_launcher_refuses_units_that_are_not_whole_rounds(eight, rf, wide, units):
+    """A piece begins whole units behind its first key and goes on in rounds of all waves' chunks: units of part of a round would leave keys out."""
+    if not ops.native_available():
+        pytest.skip("extension not built")
+    call = ctypes.CDLL(HIP_SO).dllm_tree_attention
+    P, I, L = ctypes.c_void_p, ctypes.c_int, ctypes.c_long
+    call.argtypes, call.restype = [P, L, L] + [P] * 13 + [I] * 15 + [ctypes.c_float, P], I
+    some, scale = 4096, 4096 if eight else None
+    run = lambda u: call(some, 512, 64, some, some, scale, scale, some, some, some, some, None, some, some, some, some,  # noqa: E731
+                         0, 1, 8, 8, 1, 64, 64, 64, 8, u, 1, 1, rf, wide, 16, 0.125, None)
+    for u in range(-64, 513, 32):
+        if u < 0 or u % units:
+            assert run(u) == -3, u

@@ -20,7 +20,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native, reference as ref
-from .kv8 import need, need_cache, need_vec
+from .kv8 import need, need_cache, need_vec, overlap
 
 MAX_NODES = 1024    # of a tree
 
@@ -68,7 +68,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
              "mask: contiguous int32 [T, words]")
     if out is not None:
         need(out.shape == q.shape and out.dtype == torch.bfloat16 and out.is_contiguous(), "out: contiguous bfloat16 like q, 16-byte aligned")
-        need(T == 0 or out.data_ptr() != q.data_ptr(), "out overlaps q")
+        need(T == 0 or not overlap(out, q), "out overlaps q")
     o = ref.tree_attention(q, k_cache, v_cache, block_tables, seq_qstart, seq_qlen, seq_ctx, mask, scale, k_scale, v_scale)
     if out is None:
         return o

@@ -34,6 +34,12 @@ def need(cond: bool, what: str) -> None:
         raise ValueError(what)
 
 
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of at least one value lie in common bytes (from their first to their last)."""
+    ends = [(t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * m for n, m in zip(t.shape, t.stride()))) * t.element_size()) for t in (a, b)]
+    return ends[0][0] < ends[1][1] and ends[1][0] < ends[0][1]
+
+
 def need_vec(t: torch.Tensor, name: str, n: int, like: torch.Tensor) -> None:
     need(t.device == like.device, f"{name} is on another device")
     need(t.dtype == torch.int32 and t.shape == (n,) and t.is_contiguous(), f"{name}: contiguous int32 [{n}]")

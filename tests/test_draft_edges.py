@@ -39,3 +39,17 @@ def test_the_launcher_refuses_units_that_are_not_whole_rounds(eight, rf, wide, u
     for u in range(-64, 513, 32):
         if u < 0 or u % units:
             assert run(u) == -3, u
+
+
+def test_attention_refuses_an_output_that_overlaps_its_queries():
+    s = step([(4, 20)], 8, 2, 64, False, "chain", 1)
+    for rows in (0, 1, 3):
+        both = torch.zeros(4 + rows, 8, 64, dtype=torch.bfloat16)
+        both[rows:] = s["q"]
+        for q, out in ((both[rows:], both[:4]), (both[:4], both[rows:])):
+            with pytest.raises(ValueError, match="overlaps"):
+                attend(dict(s, q=q), out=out)
+    room = torch.zeros(8, 8, 64, dtype=torch.bfloat16)              # beside each other in one tensor
+    room[:4] = s["q"]
+    attend(dict(s, q=room[:4]), out=room[4:])
+    assert torch.equal(room[4:], attend(s))

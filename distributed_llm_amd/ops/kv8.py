@@ -87,6 +87,7 @@ def rope_and_cache(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Te
          "cos_sin: contiguous float32 [max_pos, d]")
     if q_out is not None:
         need(q_out.shape == (T, nq, d) and q_out.dtype == torch.bfloat16 and q_out.is_contiguous(), "q_out: contiguous bfloat16 [T, nq, d], 16-byte aligned")
+        need(q_out.numel() == 0 or not overlap(q_out, qkv), "q_out overlaps qkv")
     need(T == 0 or blocks >= 1, "the cache has no blocks")
     q = ref.kv8_rope(qkv, positions, cos_sin, slots, cache, nq, nkv, d)
     return q if q_out is None else q_out.copy_(q)

@@ -6,7 +6,7 @@ import torch
 
 from distributed_llm_amd import ops
 from distributed_llm_amd._build import HIP_SO
-from draft_cases import attend, step
+from draft_cases import attend, i32, step
 
 
 @pytest.mark.parametrize("eight", [False, True])
@@ -53,3 +53,15 @@ def test_attention_refuses_an_output_that_overlaps_its_queries():
     room[:4] = s["q"]
     attend(dict(s, q=room[:4]), out=room[4:])
     assert torch.equal(room[4:], attend(s))
+
+
+def test_rope_and_cache_refuses_queries_that_overlap_its_rows():
+    cache, cs, at = ops.kv8.alloc(4, 2, 64), ops.rope_cos_sin(8, 64, 1e4), i32([0, 1, 2])
+    room = torch.ones(3 * 8 * 64 + 3 * 4 * 64, dtype=torch.bfloat16)
+    qkv = room[:3 * 8 * 64].view(3, 512)
+    for start in (0, 64, 3 * 8 * 64 - 8):
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.kv8.rope_and_cache(qkv, at, cs, at, cache, 4, 2, 64, q_out=room[start:start + 3 * 4 * 64].view(3, 4, 64))
+    q = ops.kv8.rope_and_cache(qkv, at, cs, at, cache, 4, 2, 64, q_out=room[3 * 8 * 64:].view(3, 4, 64))
+    assert torch.equal(q, ops.kv8.rope_and_cache(qkv, at, cs, at, cache, 4, 2, 64))
+    ops.kv8.rope_and_cache(qkv, at, cs, at, cache, 0, 2, 64, q_out=room[:0].view(3, 0, 64))      # no value to overlap

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from distributed_llm_amd import ops
-from draft_cases import attend, i32, step, to
+from draft_cases import BS, attend, attention64, i32, step, to, visible
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -84,3 +84,58 @@ def test_no_key_at_all_gives_rows_of_zeros(eight, d, what):
             assert not attend(h)[:76].any()
             outs.append(out.cpu())
         assert torch.equal(*outs) and not outs[1][:76].any() and bool((outs[1][76:] == 7.0).all())
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("seqs", [[(40, 1190), (3, 37)], [(5, 1190), (3, 37)], [(1, 1190), (1, 37)]])
+def test_an_infinity_beside_a_page_outside_the_pool(eight, d, seqs):
+    """V of a committed key whose chunk lacks a page, long before the drafted ones: every row of the sequence gets it, no other row does; a NaN of a
+    drafted key reaches its own branch alone."""
+    s = step(seqs, 8, 2, d, eight, "tree", 23)
+    n, c = seqs[0]
+    see = [visible(s, b) for b in range(2)]
+    see[0][:, 16 * BS:17 * BS] = False
+    want, bound = attention64(s, see)
+    s["table"][0, 16] = -5
+    page, off = int(s["table"][0, 17]), 3                       # key 275, at dim 9
+    s["v"].view(torch.uint8 if eight else torch.bfloat16)[page, :, 9, off] = 0x7F if eight else -math.inf
+    got = attend(to(s, DEV)).cpu()
+    hit = got[:n, :, 9].float()
+    assert bool((hit.isnan() if eight else hit == -math.inf).all())
+    rest = torch.ones_like(got, dtype=torch.bool)
+    rest[:n, :, 9] = False
+    assert bool(((got.double() - want).abs() <= bound)[rest].all())
+    if n < 2:
+        return
+    at = c - 1                                                  # the last node: no node is behind it
+    page, off = int(s["table"][0, at // BS]), at % BS
+    s["v"].view(torch.uint8 if eight else torch.bfloat16)[page, :, 20, off] = 0x7F if eight else math.nan
+    got = attend(to(s, DEV)).cpu()
+    assert got[n - 1, :, 20].isnan().all()
+    rest[n - 1, :, 20] = False
+    assert bool(((got.double() - want).abs() <= bound)[rest].all())
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("nodes", [1, 12, 40])
+def test_a_nan_of_a_drafted_token_does_not_hold_up_the_batch(eight, nodes):
+    """One broken sequence of 30000 keys: what is looked at again are its drafted keys, not its context (that took 40 times a call's time and more; four
+    times are allowed here)."""
+    s = to(step([(nodes, 30000), (nodes, 900), (nodes, 77)], 8, 2, 128, eight, "tree", 24), DEV)
+
+    def time():
+        took = []
+        for _ in range(8):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            attend(s, max_qlen=nodes)
+            b.record()
+            torch.cuda.synchronize()
+            took.append(a.elapsed_time(b))
+        return sorted(took)[3]
+    clean = time()
+    page, off = int(s["table"][0, 29999 // BS]), 29999 % BS
+    s["v"].view(torch.uint8 if eight else torch.bfloat16)[page, :, :, off] = 0x7F if eight else math.nan
+    broken = time()
+    assert broken < 4 * clean, f"{1e3 * clean:.0f} us, with a NaN {1e3 * broken:.0f}"

@@ -140,12 +140,15 @@ Tensor tree_attention(Tensor q, Tensor k, Tensor v, Tensor bt, Tensor qstart, Te
   // 113 / 116 / 118 (0 / 1 / 2 units where contexts are shorter: 512 of 200 to 1000 keys, 4 kv heads of 64, 68 / 65 / 65; 2000 of 100 to 400 146 / 141 / 140).
   // With units of 256 keys and no way 82, 100, 37, 113.  Parts of 512 keys and more from 4096 on: one sequence of 16000 65 -> 55.  A context of up to
   // 512 keys is one unit, not split: one launch (us in a graph with a bound of 256 / 512 / 1024 keys: one chat of 437, masks beside it, 10.7 / 9.0 / 9.0; 64 of
-  // 300 to 500 20 / 16.5 / 16.4; one of 800 and 40 nodes 22 / 22 / 33; 512 of up to 1000 and 5 nodes 86 / 86 / 101).
-  int64_t ulen = keys <= 512 ? 0 : wide ? 64 : c.eight && rf == 1 ? 256 : 128;
+  // 300 to 500 20 / 16.5 / 16.4; one of 800 and 40 nodes 22 / 22 / 33; 512 of up to 1000 and 5 nodes 86 / 86 / 101).  Parts are then of whole row blocks, as
+  // uneven as their lengths, so from more than five row blocks a workgroup on contexts of more than 256 keys are cut after all.  us whole / cut, 8 kv heads of
+  // 128, one token, bf16 and e4m3: 96 sequences of 500 keys 48 / 50 and 29 / 32, 128 of 300 to 500 48 / 54 and 31 / 33, of 20 to 500 27 / 27 and 21 / 27, 256 of
+  // those 59 / 53 and 39 / 42, 384 91 / 76 and 62 / 61, 512 117 / 96 and 84 / 79; 384 of 500 159 / 162 and 105 / 109.  48 trees of 40 nodes 36 / 51.
+  const int64_t listed = c.nkv * (T * G / R + S);      // row blocks, at most, however long the longest
+  int64_t ulen = keys <= 256 || (keys <= 512 && std::min(blocks, listed) <= 5 * nwg) ? 0 : wide ? 64 : c.eight && rf == 1 ? 256 : 128;
   const int64_t way = wide ? 4 : rf > 1 ? 3 : c.eight || keys <= 4096 ? 1 : 0, least = ulen ? (keys > 4096 ? 512 : 256) / ulen : 1;
   // the list of units is counted in 32 bits
   NEED(c.nkv < (1 << 20), "tree_attention: too many heads");
-  const int64_t listed = c.nkv * (T * G / R + S);
   NEED(T * nq <= 0x7fffffff && listed < (1 << 30), "tree_attention: too many");
   while (ulen && listed * (max_blocks * BS / ulen + 1 + way) >= (1 << 30)) ulen *= 2;
   nwg = std::min(nwg, (blocks * (ulen ? (keys + ulen - 1) / ulen : 1) + 7) / 8 * 8);

@@ -1,11 +1,12 @@
 """Drafted tokens at the edges of what their calls allow: kernels against their definitions and against the CPU forms."""
 import math
+import random
 
 import pytest
 import torch
 
 from distributed_llm_amd import ops
-from draft_cases import BS, attend, attention64, i32, step, to, visible
+from draft_cases import BS, attend, attention64, dense, i32, step, to, visible
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -139,3 +140,34 @@ def test_a_nan_of_a_drafted_token_does_not_hold_up_the_batch(eight, nodes):
     s["v"].view(torch.uint8 if eight else torch.bfloat16)[page, :, :, off] = 0x7F if eight else math.nan
     broken = time()
     assert broken < 4 * clean, f"{1e3 * clean:.0f} us, with a NaN {1e3 * broken:.0f}"
+
+
+def heads_at_once(s):
+    """``attention64`` for many sequences: the same definition and bound, all heads of a sequence in one product."""
+    T, nq, d = s["q"].shape
+    out, bound = torch.zeros(T, nq, d, dtype=torch.float64), torch.zeros(T, nq, d, dtype=torch.float64)
+    for b in range(s["table"].shape[0]):
+        q0, n, c = int(s["qstart"][b]), int(s["qlen"][b]), int(s["ctx"][b])
+        k, v = dense(s, b)
+        x = s["q"][q0:q0 + n].double().transpose(0, 1).reshape(k.shape[0], -1, d)                # [nkv, G n, d]
+        hidden = ~visible(s, b).repeat(nq // k.shape[0], 1)
+        w = torch.softmax((x @ k.transpose(1, 2) / math.sqrt(d)).masked_fill(hidden, -math.inf), -1)
+        ds = (d + 3) * 2.0 ** -24 * (x.abs() @ k.abs().transpose(1, 2) / math.sqrt(d)).masked_fill(hidden, 0.0).amax(-1, keepdim=True)
+        e = (2.0 ** -8 + 2 * ds + (2 * c + 16) * 2.0 ** -24) * (w @ v.abs())
+        for to, x in ((out, w @ v), (bound, e + 2.0 ** -8 * ((w @ v).abs() + e) + 1e-30)):
+            to[q0:q0 + n] = x.view(nq, n, d).transpose(0, 1)
+    return out, bound
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("batch,nodes", [(75, 12), (90, 1), (90, 12)])
+def test_many_short_contexts(eight, batch, nodes):
+    """Below and above the number of row blocks from which contexts of up to 512 keys are cut, lengths of their own; with the longest ones given and without."""
+    rng = random.Random(batch)
+    s = step([(min(nodes, c), c) for c in (rng.randrange(1, 512) for _ in range(batch))], 64, 32, 64, eight, "tree", 25)
+    want, bound = heads_at_once(s)
+    h = to(s, DEV)
+    for kw in ({}, dict(max_qlen=nodes, max_ctx=511)):
+        got = attend(h, **kw)
+        assert bool(((got.double().cpu() - want).abs() <= bound).all())
+        assert torch.equal(got, attend(h, **kw))

@@ -45,8 +45,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     """Attention of new tokens ``q`` [T, nq, d] (bf16, head_dim 64, 96 or 128) over the paged cache, bf16 or, with its scales, 8-bit.
 
     A token sees the ``seq_ctx - seq_qlen`` keys before its sequence's new ones, and of those the ones that ``mask`` (``tree_mask``) names; without a mask
-    itself and those before it (a chain, a prompt's rows, a single token).  A row that sees nothing is zero; what a row does not see does not reach it,
-    NaN and infinities included, nor do keys of pages outside the pool.  Any number of query heads a kv head.  Rows of ``q`` that belong to no sequence are
+    itself and those before it (a chain, a prompt's rows, a single token).  A row that sees nothing, or scores of minus infinity alone, is zero; what a row does not
+    see does not reach it, NaN and infinities included, nor do keys of pages outside the pool.  Any number of query heads a kv head.  Rows of ``q`` that belong to no sequence are
     not written.  ``max_qlen``, ``max_ctx``: the longest, where the host knows them (0: it does not); they pick the launch, never the result's rows."""
     scale = (1.0 / math.sqrt(q.shape[-1])) if scale is None else scale
     ext = _native(q)

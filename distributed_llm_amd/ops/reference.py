@@ -1232,7 +1232,8 @@ def tree_attention(q, k_cache, v_cache, block_tables, seq_qstart, seq_qlen, seq_
             if not bool(see.any()):
                 continue
             x = q[q0 + i].to(wide).view(nkv, G, d)
-            w = torch.softmax((x @ k[:, see].transpose(1, 2)) * scale, -1)
+            sc = (x @ k[:, see].transpose(1, 2)) * scale
+            w = torch.where((sc == -math.inf).all(-1, keepdim=True), 0.0, torch.softmax(sc, -1))
             out[q0 + i] = (w @ v[:, see]).reshape(nq, d).to(q.dtype)
     return out
 

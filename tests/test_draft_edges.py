@@ -6,7 +6,7 @@ import torch
 
 from distributed_llm_amd import ops
 from distributed_llm_amd._build import HIP_SO
-from draft_cases import attend, i32, step
+from draft_cases import BS, attend, attention64, i32, step, to
 
 
 @pytest.mark.parametrize("eight", [False, True])
@@ -65,3 +65,22 @@ def test_rope_and_cache_refuses_queries_that_overlap_its_rows():
     q = ops.kv8.rope_and_cache(qkv, at, cs, at, cache, 4, 2, 64, q_out=room[3 * 8 * 64:].view(3, 4, 64))
     assert torch.equal(q, ops.kv8.rope_and_cache(qkv, at, cs, at, cache, 4, 2, 64))
     ops.kv8.rope_and_cache(qkv, at, cs, at, cache, 0, 2, 64, q_out=room[:0].view(3, 0, 64))      # no value to overlap
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("keys", [9, 700])
+def test_a_row_whose_scores_are_all_minus_infinity_is_zero(device, eight, keys):
+    """A score of minus infinity weighs nothing, as a key that is not seen; of plus infinity the row is NaN.  Keys of -3e38 in 64 dims overflow."""
+    s = step([(2, keys), (3, 40)], 8, 2, 64, eight, "chain", 6)
+    want, bound = attention64(s)
+    mine = s["table"][0, :-(-keys // BS)].long()
+    if eight:
+        s["ks"][mine] = 3e38 / 448
+        s["k"].view(torch.uint8)[mine] = 0xFE                       # -448
+    else:
+        s["k"][mine] = -3e38
+    s["q"][0], s["q"][1] = 2.0, -2.0
+    got = attend(to(s, device)).cpu()
+    assert not got[0].any() and got[1].isnan().all()
+    assert bool(((got[2:].double() - want[2:]).abs() <= bound[2:]).all())

@@ -171,3 +171,34 @@ def test_many_short_contexts(eight, batch, nodes):
         got = attend(h, **kw)
         assert bool(((got.double().cpu() - want).abs() <= bound).all())
         assert torch.equal(got, attend(h, **kw))
+
+
+@pytest.mark.parametrize("d,hint", [(64, 0), (64, 9), (128, 9), (96, 0)])
+def test_every_part_longer_than_its_window_of_pages(d, hint):
+    """430 sequences of 20000 keys, each with an order of pages of its own: a workgroup's part passes 16384 keys of one row block, from a context's first
+    key on or from inside it, and its pages are looked up again on the way.  All rows are compared; then with two pages of every sequence outside the
+    pool, most of them past a window's first 1024.  Bounds as attention64's."""
+    n, ctx, qlen, blocks = 430, 20000, 9, 1250
+    s = to(step([(qlen, ctx)], 4, 1, d, False, "chain", 18), DEV)
+    g = torch.Generator().manual_seed(2)
+    s["q"] = (1.5 * torch.randn(n * qlen, 4, d, generator=g)).bfloat16().to(DEV)
+    order = torch.stack([torch.randperm(blocks, generator=g) for _ in range(n)])
+    s["table"] = s["table"][0].cpu()[order].contiguous().to(DEV)
+    s["qstart"], s["qlen"], s["ctx"] = i32(list(range(0, n * qlen, qlen)), DEV), i32([qlen] * n, DEV), i32([ctx] * n, DEV)
+    k, v = (s["k"][:, 0].double(), s["v"][:, 0].transpose(1, 2).double())                       # [pages, 16, d]
+    see = torch.arange(ctx, device=DEV)[None] <= ctx - qlen + torch.arange(qlen, device=DEV)[:, None]
+    away = torch.stack([torch.randint(0, blocks, (n,), generator=g), torch.randint(1024, blocks, (n,), generator=g)], 1).to(DEV)
+    holed = s["table"].scatter(1, away, torch.where(away % 2 == 0, -1, s["k"].shape[0]).int())
+    for table in (s["table"], holed):
+        got = attend(dict(s, table=table), max_qlen=hint).double()
+        for b in range(n):
+            pages = s["table"][b].long()
+            kk, vv = k[pages].reshape(ctx, d), v[pages].reshape(ctx, d)
+            seen = see & ((table[b] >= 0) & (table[b] < s["k"].shape[0])).repeat_interleave(BS)[None]
+            x = s["q"][b * qlen:(b + 1) * qlen].double().transpose(0, 1)                        # [4, qlen, d]
+            w = torch.softmax((x @ kk.T / math.sqrt(d)).masked_fill(~seen, -math.inf), -1)
+            ds = (d + 3) * 2.0 ** -24 * (x.abs() @ kk.abs().T / math.sqrt(d)).masked_fill(~seen, 0.0).amax(-1, keepdim=True)
+            o = w @ vv
+            e = (2.0 ** -8 + 2 * ds + (2 * ctx + 16) * 2.0 ** -24) * (w @ vv.abs())
+            off = (got[b * qlen:(b + 1) * qlen].transpose(0, 1) - o).abs()
+            assert bool((off <= e + 2.0 ** -8 * (o.abs() + e)).all()), b

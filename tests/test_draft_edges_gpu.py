@@ -202,3 +202,38 @@ def test_every_part_longer_than_its_window_of_pages(d, hint):
             e = (2.0 ** -8 + 2 * ds + (2 * ctx + 16) * 2.0 ** -24) * (w @ vv.abs())
             off = (got[b * qlen:(b + 1) * qlen].transpose(0, 1) - o).abs()
             assert bool((off <= e + 2.0 ** -8 * (o.abs() + e)).all()), b
+
+
+# ------------------------------------------------------------------------------------------------ vocabularies past 4096 tokens a part
+BIG = 4096 * 256 + 3
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_vocabularies_of_more_than_a_million(drawn, dtype):
+    """Parts of 8192 tokens, 32 a thread, the last part of three: draws all over the vocabulary, of flat and of peaked rows."""
+    g = torch.Generator().manual_seed(7)
+    n = 6
+    logits = 3 * torch.randn(2 * n, BIG, generator=g)
+    target = torch.softmax(logits, -1)
+    target[::4] = 1.0 / BIG
+    draft = torch.softmax(logits + torch.randn(2 * n, BIG, generator=g), -1) if drawn else None
+    tokens = torch.multinomial(target, 1, generator=g)[:, 0].int()
+    u = torch.rand(2 * n, generator=g)
+    u[::2] = (torch.arange(n) + 0.37) / n                       # the roots': the next token's
+    s = dict(target=target.to(dtype), tokens=tokens, uniform=u, qstart=i32(list(range(0, 2 * n, 2))), qlen=i32([2] * n),
+             draft=None if draft is None else draft.to(dtype))
+    _, token, _ = verified(s, 2)
+    assert len(set(token)) == n
+
+
+def test_tokens_at_the_ends_of_threads_and_parts():
+    """One row each with all its weight in two places, the draw of the second: the first and the last sixteen of a thread's tokens, a part's ends and the
+    three tokens of the last part."""
+    places = [0, 15, 16, 31, 32, 8191, 8192, 8192 + 17, 100 * 8192 + 40, BIG - 4, BIG - 3, BIG - 2, BIG - 1]
+    target = torch.zeros(len(places), BIG)
+    for i, at in enumerate(places):
+        target[i, max(at - 3, 0)], target[i, at] = 0.25, 0.5
+    n = len(places)
+    _, token, _ = verified(dict(target=target, tokens=i32([0] * n), uniform=torch.full((n,), 0.75), qstart=i32(list(range(n))), qlen=i32([1] * n)), 1)
+    assert token == places

@@ -20,7 +20,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native, reference as ref
-from .kv8 import need, need_cache, need_vec, overlap
+from .kv8 import need, need_cache, need_device, need_vec, overlap
 
 MAX_NODES = 1024    # of a tree
 
@@ -58,15 +58,18 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _, nkv, dim = need_cache(k_cache, v_cache, k_scale, v_scale, q)
     need(dim == d and d in (64, 96, 128), "head_dim must be 64, 96 or 128, and the cache's")
     need(nkv >= 1 and nq >= 1 and nq % nkv == 0, "query heads must be a multiple of the cache's")
-    need(block_tables.device == q.device and block_tables.dim() == 2 and block_tables.dtype == torch.int32 and block_tables.is_contiguous(),
+    need_device(block_tables, "block_tables", q)
+    need(block_tables.dim() == 2 and block_tables.dtype == torch.int32 and block_tables.is_contiguous(),
          "block_tables: contiguous int32 [num_seqs, max_blocks]")
     for t, name in ((seq_qstart, "seq_qstart"), (seq_qlen, "seq_qlen"), (seq_ctx, "seq_ctx")):
         need_vec(t, name, block_tables.shape[0], q)
     need(max_qlen >= 0 and max_ctx >= 0, "max_qlen and max_ctx: 0 (unknown) or more")
     if mask is not None:
-        need(mask.device == q.device and mask.dim() == 2 and mask.dtype == torch.int32 and mask.is_contiguous() and mask.shape[0] == T and mask.shape[1] >= 1,
+        need_device(mask, "mask", q)
+        need(mask.dim() == 2 and mask.dtype == torch.int32 and mask.is_contiguous() and mask.shape[0] == T and mask.shape[1] >= 1,
              "mask: contiguous int32 [T, words]")
     if out is not None:
+        need_device(out, "out", q)
         need(out.shape == q.shape and out.dtype == torch.bfloat16 and out.is_contiguous(), "out: contiguous bfloat16 like q, 16-byte aligned")
         need(T == 0 or not overlap(out, q), "out overlaps q")
     o = ref.tree_attention(q, k_cache, v_cache, block_tables, seq_qstart, seq_qlen, seq_ctx, mask, scale, k_scale, v_scale)
@@ -98,6 +101,7 @@ def verify(target: torch.Tensor, tokens: torch.Tensor, uniform: torch.Tensor, se
          "target: float32 or bfloat16 [T, vocab]")
     T, S = target.shape[0], seq_qstart.numel()
     need_vec(tokens, "tokens", T, target)
+    need_device(uniform, "uniform", target)
     need(uniform.dtype == torch.float32 and uniform.shape == (T,) and uniform.is_contiguous(), "uniform: contiguous float32 [T]")
     need_vec(seq_qstart, "seq_qstart", S, target)
     need_vec(seq_qlen, "seq_qlen", S, target)
@@ -106,6 +110,7 @@ def verify(target: torch.Tensor, tokens: torch.Tensor, uniform: torch.Tensor, se
     if parents is not None:
         need_vec(parents, "parents", T, target)
     if draft is not None:
+        need_device(draft, "draft", target)
         need(draft.shape == target.shape and draft.dtype == target.dtype and (draft.stride(1) == 1 or draft.shape[1] == 1), "draft: like target")
     need(S <= 65535, "at most 65535 sequences")
     return ref.verify_drafts(target, tokens, uniform, seq_qstart, seq_qlen, max_nodes, parents, draft)
@@ -122,10 +127,12 @@ def keep(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tenso
     need(k_cache.dim() in (4, 5), "caches: one layer's or [layers, ...]")
     _, _, d = need_cache(k_cache, v_cache, k_scale, v_scale, k_cache, k_cache.dim() - 4)
     need(16 <= d <= 128 and d % 16 == 0, "head_dim must be a multiple of 16, at most 128")
+    need_device(block_tables, "block_tables", k_cache)
     need(block_tables.dim() == 2 and block_tables.dtype == torch.int32 and block_tables.is_contiguous(), "block_tables: contiguous int32 [num_seqs, max_blocks]")
     S = block_tables.shape[0]
     for t, name in ((seq_qlen, "seq_qlen"), (seq_ctx, "seq_ctx"), (accepted, "accepted")):
         need_vec(t, name, S, k_cache)
+    need_device(path, "path", k_cache)
     need(path.dim() == 2 and path.dtype == torch.int32 and path.is_contiguous() and path.shape[0] == S and path.shape[1] >= 1,
          "path: contiguous int32 [num_seqs, max_nodes]")
     need(S <= 65535, "at most 65535 sequences")

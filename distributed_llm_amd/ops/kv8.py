@@ -34,6 +34,10 @@ def need(cond: bool, what: str) -> None:
         raise ValueError(what)
 
 
+def need_device(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
+    need(t.device == like.device, f"{name} is on another device")
+
+
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors of at least one value lie in common bytes (from their first to their last)."""
     ends = [(t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * m for n, m in zip(t.shape, t.stride()))) * t.element_size()) for t in (a, b)]
@@ -41,7 +45,7 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def need_vec(t: torch.Tensor, name: str, n: int, like: torch.Tensor) -> None:
-    need(t.device == like.device, f"{name} is on another device")
+    need_device(t, name, like)
     need(t.dtype == torch.int32 and t.shape == (n,) and t.is_contiguous(), f"{name}: contiguous int32 [{n}]")
 
 
@@ -83,9 +87,11 @@ def rope_and_cache(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Te
     need(n == nkv and dim == d and nq >= 0 and nkv >= 1 and qkv.shape[1] >= (nq + 2 * nkv) * d, "qkv and cache disagree on heads or head_dim")
     need_vec(positions, "positions", T, qkv)
     need_vec(slots, "slots", T, qkv)
+    need_device(cos_sin, "cos_sin", qkv)
     need(cos_sin.dim() == 2 and cos_sin.dtype == torch.float32 and cos_sin.is_contiguous() and cos_sin.shape[1] == d and cos_sin.shape[0] >= 1,
          "cos_sin: contiguous float32 [max_pos, d]")
     if q_out is not None:
+        need_device(q_out, "q_out", qkv)
         need(q_out.shape == (T, nq, d) and q_out.dtype == torch.bfloat16 and q_out.is_contiguous(), "q_out: contiguous bfloat16 [T, nq, d], 16-byte aligned")
         need(q_out.numel() == 0 or not overlap(q_out, qkv), "q_out overlaps qkv")
     need(T == 0 or blocks >= 1, "the cache has no blocks")
@@ -101,6 +107,7 @@ def write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Cache) -
     for t in (k, v):
         need(t.dim() == 3 and t.dtype == torch.bfloat16 and t.shape == k.shape and t.stride(2) == 1 and (t.stride(1) == t.shape[2] or t.shape[1] == 1) and
              t.stride(0) % 8 == 0, "k, v: bfloat16 [T, nkv, d] with rows of 16-byte alignment")
+    need_device(v, "v", k)
     blocks, nkv, d = _need_kv8(cache, k)
     need(nkv == k.shape[1] and d == k.shape[2] and nkv >= 1, "k, v and cache disagree on heads or head_dim")
     need_vec(slots, "slots", k.shape[0], k)

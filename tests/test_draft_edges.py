@@ -84,3 +84,37 @@ def test_a_row_whose_scores_are_all_minus_infinity_is_zero(device, eight, keys):
     got = attend(to(s, device)).cpu()
     assert not got[0].any() and got[1].isnan().all()
     assert bool(((got[2:].double() - want[2:]).abs() <= bound[2:]).all())
+
+
+def test_tensors_of_another_device_are_refused():
+    """As the kernels' checks have it; here a device without data."""
+    away = lambda t: t.to("meta")  # noqa: E731
+    s = step([(4, 20)], 8, 2, 64, True, "tree", 1)
+    for t in ("k", "vs", "table", "qlen", "mask"):
+        with pytest.raises(ValueError, match="another device"):
+            attend(dict(s, **{t: away(s[t])}))
+    with pytest.raises(ValueError, match="another device"):
+        attend(s, out=away(s["q"]))
+    p, tok, u, n = torch.full((3, 8), 0.125), i32([0, 1, 2]), torch.rand(3), i32([3])
+    good = dict(target=p, tokens=tok, uniform=u, seq_qstart=i32([0]), seq_qlen=n, max_nodes=3)
+    for bad in (dict(tokens=away(tok)), dict(uniform=away(u)), dict(seq_qlen=away(n)), dict(parents=away(tok)), dict(draft=away(p))):
+        with pytest.raises(ValueError, match="another device"):
+            ops.draft.verify(**dict(good, **bad))
+    path = i32([[0, 2, 3, -1]])
+    good = dict(k_cache=s["k"], v_cache=s["v"], block_tables=s["table"], seq_qlen=s["qlen"], seq_ctx=s["ctx"], path=path, accepted=i32([2]), k_scale=s["ks"],
+                v_scale=s["vs"])
+    for t in ("v_cache", "block_tables", "seq_ctx", "path", "accepted", "k_scale"):
+        with pytest.raises(ValueError, match="another device"):
+            ops.draft.keep(**dict(good, **{t: away(good[t])}))
+    c, qkv, cs = ops.kv8.alloc(4, 2, 64), torch.zeros(3, 512, dtype=torch.bfloat16), ops.rope_cos_sin(8, 64, 1e4)
+    for args in ((qkv, away(tok), cs, tok, c), (qkv, tok, away(cs), tok, c), (qkv, tok, cs, away(tok), c), (qkv, tok, cs, tok, c._replace(v=away(c.v)))):
+        with pytest.raises(ValueError, match="another device"):
+            ops.kv8.rope_and_cache(*args, 4, 2, 64)
+    with pytest.raises(ValueError, match="another device"):
+        ops.kv8.rope_and_cache(qkv, tok, cs, tok, c, 4, 2, 64, q_out=away(torch.zeros(3, 4, 64, dtype=torch.bfloat16)))
+    x = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    for args in ((x, away(x), tok, c), (x, x, away(tok), c)):
+        with pytest.raises(ValueError, match="another device"):
+            ops.kv8.write(*args)
+    with pytest.raises(ValueError, match="another device"):
+        ops.kv8.read(c, away(tok))

@@ -137,7 +137,9 @@ Tensor tree_attention(Tensor q, Tensor k, Tensor v, Tensor bt, Tensor qstart, Te
   // Keys of a unit (of whole rounds of a workgroup's chunks), units that a row block's way in and out counts for, and units of a part, at least: short
   // parts of long contexts leave many pieces to join.  us with a way of 0 / 2 / 3 / 4 / 6 units: ragged trees of 80 to 160 rows 94 / 78 / 75 / 74 / 75, 160
   // rows of a chain 108 / 91 / 87 / 86 / 92; 48 rows over e4m3 39 / 37 / 35 / 35 / 36; 16 rows are bound by memory, 64 single tokens of up to 6000 keys
-  // 113 / 116 / 118 (0 / 1 / 2 units where contexts are shorter: 512 of 200 to 1000 keys, 4 kv heads of 64, 68 / 65 / 65; 2000 of 100 to 400 146 / 141 / 140).
+  // 113 / 116 / 118 (0 / 1 / 2 units where contexts are shorter: 512 of 200 to 1000 keys, 4 kv heads of 64, 68 / 65 / 65; 2000 of 100 to 400 146 / 141 / 140;
+  // 0 / 1 for even and for ragged contexts: 32 of 1500 45 / 48, of 200 to 1500 24 / 24; 8 of 1000 14 / 16, of 300 to 1000 15 / 13; 128 of 1500 149 / 150, of 200
+  // to 1500 88 / 85, 4 kv heads of 64 48 / 49 and 25 / 23).
   // With units of 256 keys and no way 82, 100, 37, 113.  Parts of 512 keys and more from 4096 on: one sequence of 16000 65 -> 55.  A context of up to
   // 512 keys is one unit, not split: one launch (us in a graph with a bound of 256 / 512 / 1024 keys: one chat of 437, masks beside it, 10.7 / 9.0 / 9.0; 64 of
   // 300 to 500 20 / 16.5 / 16.4; one of 800 and 40 nodes 22 / 22 / 33; 512 of up to 1000 and 5 nodes 86 / 86 / 101).  Parts are then of whole row blocks, as

@@ -218,7 +218,7 @@ template <class T> static __device__ __forceinline__ void tree_walk(const Verify
 // The walk, in every workgroup of a sequence (a few dependent loads: it costs less than a launch of its own), then the weights' sum of this one's part of the
 // vocabulary; the token is found by a second launch.  Node i is accepted where u q(x) < p(x) (drawn from q), or u m < p(x), m = 1 less what its earlier
 // siblings held (given candidates): products of f32 and f64 values, exact or rounded once, so a token does not hang on the order of sums.
-// 48 chains, 128256 tokens: 13.5 us of the walk's four trips to memory and 49 MB (3.6 TB/s), 6.7 for the second launch; one chain of 32000: 6.0 and 5.6.
+// 48 chains, 128256 tokens: 13 us of the walk's four trips to memory and 49 MB (3.8 TB/s), 7.5 for the second launch; one chain of 32000: 6.0 and 5.8.
 template <class T> __global__ void __launch_bounds__(NTH) verify_walk_kernel(VerifyArgs a) {
   __shared__ VerifySmem sm;
   const int s = blockIdx.y, tid = threadIdx.x, q0 = a.qstart[s];
@@ -237,7 +237,7 @@ template <class T> __global__ void __launch_bounds__(NTH) verify_walk_kernel(Ver
   bool refused;
   const int v0 = blockIdx.x * a.part, v1 = v0 + min(a.V - v0, a.part);      // (a whole last part may end past 2^31)
   if (n <= 64) {
-    // a lane a node, in every wave by itself, without LDS (trees of 40 nodes: 16 us of a launch in LDS, 11 so)
+    // a lane a node, in every wave by itself, without LDS (trees of 40 nodes: 16 us of a launch in LDS, 9 so)
     const int i = tid & 63, x = i < n ? a.tokens[q0 + i] : -1, par = i < n ? parent_of(a, q0, i) : -3;
     const bool real = par >= 0 && x >= 0 && x < a.V;
     double px = real ? (double)val<T>(target + (long)(q0 + par) * a.target_ld + x) : 0.0, mass = 1.0;
@@ -446,7 +446,7 @@ struct KeepArgs {
 };
 
 // V is a column of a transposed block, two bytes of every 32: a move touches lines of 32 d bytes for 2 d, which bounds it (32 sequences, 32 layers of 8 heads of
-// 128: 25 MB moved, about 200 touched, 30 us; four heads a workgroup 36).
+// 128: 25 MB moved, about 100 MB of lines, each counted once however many of its tokens move, 30 us; four heads a workgroup 36).
 // A workgroup: one sequence, layer and kv head.  Path indices rise and node path[j] goes to place j <= path[j]: sixteen tokens at a time are
 // read, then written, and what is written lies ahead of every later source.  E: bytes of a value.
 template <int E> __global__ void __launch_bounds__(NTH) keep_kernel(KeepArgs a) {

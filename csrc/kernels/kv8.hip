@@ -2,8 +2,9 @@
 //   scale = top / 448, code = e4m3(448 x / top), top = max |x|, at least 2^-100.
 // Layouts as the bf16 cache's: K [blocks, nkv, 16, d], V [blocks, nkv, d, 16], scales [blocks, nkv, 16].
 //
-// The quotient is rounded to f32 once ahead of the code (448 = 0.875 * 512, so that nothing overflows): a bf16 value that lies half way between
-// two codes stays there and goes to the even one, as in exact arithmetic.  A vector with an infinity or NaN reads back as NaN.
+// 448 = 0.875 * 512, so that nothing overflows.  0.875 x is exact for a bf16 value and the quotient is rounded to f32 once ahead of the code: one that lies
+// half way between two codes stays there and goes to the even one, as in exact arithmetic.  A rotated K has 24 bits and is rounded in both steps: within
+// 2^-23 of a tie it may go to the other side, which is a code's half step either way.  A vector with an infinity or NaN reads back as NaN.
 #include "common.h"
 
 namespace {

@@ -10,14 +10,18 @@
 //
 // Few rows (up to 32; e4m3: any number, 48 at a time): a workgroup is four waves over the same 16 RF rows (heads of one kv head, tokens x group), each
 // with its own chunks.  K and V go to registers once for all rows and are never staged; the waves meet in LDS at the end.  Bound by memory: 64
-// single tokens of 500 to 6000 keys, 8 kv heads of 128, 112 us (5.2 TB/s), over e4m3 66 (4.5).  More rows: tree_wide_kernel below.
+// single tokens of 500 to 6000 keys, 8 kv heads of 128, 112 us (5.2 TB/s), over e4m3 65 (4.6).  More rows: tree_wide_kernel below.
+//
+// Weights enter the second product as bf16, half a step (2^-8) each: the product's operands have one type, and f32 ones run at a sixteenth of the rate.
+// Steps of many keys fall either way, so the output is off by 0.0022 to 0.0024 of its norm where rounding the exact result to bf16 alone makes 0.0017.
+// Scores, maxima, the sum of weights and the output's sums stay in 32 bits, pieces between launches too.
 //
 // e4m3 caches: codes become bf16 exactly (three bits behind the leading one), the key's scale multiplies its score and the value's its weight,
 // ahead of the weight's rounding to bf16; the sum of weights is of the unrounded ones.
 //
-// Split: all (sequence, kv head, row block, range of `ulen` keys) form one list, cut into equal parts for the workgroups that fit the chip at
+// Split: all (sequence, kv head, row block, range of `ulen` keys; whole contexts where they are short) form one list, cut into equal parts for the workgroups that fit the chip at
 // once; a row block counts for some units more than its keys, for the way in and out of it (queries, masks, sums).  Every workgroup finds its
-// part from the lengths on the device, so ragged batches are even, nothing is planned on the host and a captured graph takes new lengths.  A
+// part from the lengths on the device, so ragged batches whose contexts are cut are even, nothing is planned on the host and a captured graph takes new lengths.  A
 // part's first and last piece may be of a row block that others hold too: their sums go to the workspace in 32 bits and a second launch joins
 // them, in order (no atomics: the same bits every time).
 #include "common.h"

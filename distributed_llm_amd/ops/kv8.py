@@ -4,8 +4,9 @@ Half the bytes of the bf16 cache (and 4 a vector), so half the time of a decode 
 the bf16 cache's: K [num_blocks, nkv, 16, d], V [num_blocks, nkv, d, 16], scales [num_blocks, nkv, 16], slot = block * 16 + offset, negative slots
 (padding rows) are not written.  Attention over it: ``draft.tree_attention`` with the scales, for single tokens, drafted trees and the rows of a prompt.
 
-A vector's scale is its largest magnitude / 448 (2^-100 / 448 at least) and its codes are e4m3(448 x / largest), rounded to nearest even: what reads back is
-off by at most 2^-4 of the value, or 2^-10 / 448 of the vector's largest where that is more.  A vector with an infinity or NaN reads back as NaN.
+A vector's scale is its largest magnitude / 448 (2^-100 / 448 at least) and its codes are e4m3(448 x / largest), rounded to nearest even: code times scale,
+which is what attention computes with, is off by at most 2^-4 of the value, or 2^-10 / 448 of the vector's largest where that is more; ``read`` rounds it to
+bf16 once more.  A vector with an infinity or NaN reads back as NaN.
 """
 from __future__ import annotations
 

@@ -47,6 +47,9 @@ struct TreeArgs {
 
 // ---- the list of units (32-bit: the launcher makes units long enough; lengths that contradict each other end at MOST and reach no memory but their own)
 constexpr int MOST = 1 << 30;
+// Two counts of up to MOST (their sum does not fit 31 bits).
+static constexpr int add_units(int x, int y) { return (uint32_t)x + (uint32_t)y < (uint32_t)MOST ? x + y : MOST; }
+static_assert(add_units(MOST, MOST) == MOST && add_units(MOST - 1, 1) == MOST && add_units(5, 7) == 12, "counts end at MOST");
 struct Shape {
   int qlen, ctx, nb, nt;    // row blocks, and units of each: a.way for its way in and out, and its key ranges
 };
@@ -87,13 +90,13 @@ static __device__ __forceinline__ List scan_units(const TreeArgs& a, int R) {
     q.ctx = a.ctx[s];
     q.qstart = a.qstart[s];
     const Shape h = shape_of(a, q.qlen, q.ctx, R);
-    if (q.first + i < a.S) q.incl = min(q.incl + units_of(a, h), MOST);
+    if (q.first + i < a.S) q.incl = add_units(q.incl, units_of(a, h));
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     if (o < a.S) {                                            // (lanes from S on are not looked at)
       const int y = __shfl_up(q.incl, o, 64);
-      if (lane >= o) q.incl = min(q.incl + y, MOST);
+      if (lane >= o) q.incl = add_units(q.incl, y);
     }
   }
   q.total = __builtin_amdgcn_readlane(q.incl, min(a.S, 64) - 1);
